@@ -72,6 +72,21 @@ class SpecStats(C.Structure):
     _fields_ = [("attempts", C.c_uint64), ("drafted", C.c_uint64), ("accepted", C.c_uint64)]
 
 
+class PagesConfig(C.Structure):
+    """fl_pages_config."""
+
+    _fields_ = [
+        ("num_layers", C.c_int),
+        ("num_kv_heads", C.c_int),
+        ("head_dim", C.c_int),
+        ("kv_format", C.c_int),
+        ("num_pages", C.c_int),
+        ("page_size", C.c_int),
+        ("max_seqs", C.c_int),
+        ("max_seq_len", C.c_int),
+    ]
+
+
 RNG_FN = C.CFUNCTYPE(C.c_float, C.c_void_p)
 TOKEN_FN = C.CFUNCTYPE(C.c_int, C.c_uint32, C.c_size_t, C.c_void_p)
 
@@ -85,6 +100,7 @@ SIGNATURES = {
     "fl_last_error": (C.c_char_p, [vp]),
     "fl_ctx_stream": (vp, [vp]),
     "fl_sync": (i32, [vp]),
+    "fl_ctx_device": (i32, [vp]),
     "fl_set_option": (i32, [vp, i32, i32]),
     "fl_weight_upload": (i32, [vp, C.POINTER(RawWeight), C.POINTER(vp)]),
     "fl_weight_free": (None, [vp, vp]),
@@ -162,6 +178,23 @@ SIGNATURES = {
     "fl_gguf_raw_weight": (i32, [vp, C.c_char_p, C.POINTER(RawWeight)]),
     "fl_gguf_tensor_f32": (i32, [vp, C.c_char_p, vp, sz]),
     "fl_model_load_gguf": (i32, [vp, vp, i32, i32]),
+    "fl_pages_bytes": (i32, [C.POINTER(PagesConfig), C.POINTER(sz), C.POINTER(sz)]),
+    "fl_pages_create": (i32, [vp, C.POINTER(PagesConfig), vp, vp, vp, vp, C.POINTER(vp)]),
+    "fl_pages_destroy": (None, [vp]),
+    "fl_pages_fork": (i32, [vp, vp, vp, vp, i32]),
+    "fl_pages_copy": (i32, [vp, vp, vp, i32]),
+    "fl_pages_free": (i32, [vp, vp, i32]),
+    "fl_pages_truncate": (i32, [vp, vp, vp, i32]),
+    "fl_pages_extend": (i32, [vp, vp, vp, i32]),
+    "fl_pages_write": (i32, [vp, i32, i32, vp, vp, sz]),
+    "fl_pages_compact": (i32, [vp, C.POINTER(i32)]),
+    "fl_pages_read": (i32, [vp, i32, vp, vp, vp, i32, vp, vp]),
+    "fl_pages_attention": (i32, [vp, i32, vp, sz, vp, vp, i32, i32, vp]),
+    "fl_pages_len": (i32, [vp, i32]),
+    "fl_pages_free_count": (i32, [vp]),
+    "fl_pages_tables": (i32, [vp, vp, vp]),
+    "fl_pages_copies": (i32, [vp, vp, i32]),
+    "fl_pages_plan": (i32, [vp, vp, vp, i32, i32, vp, i32]),
     "fl_bench_layer_kernel": (i32, [vp, i32, i32, i32, C.POINTER(C.c_double)]),
     "fl_bench_kernel_name": (C.c_char_p, [vp, i32]),
     "fl_synth_normal": (None, [C.c_uint64, C.c_uint64, sz, f32, f32, vp]),

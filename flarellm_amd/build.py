@@ -39,8 +39,8 @@ def _run(cmd: list[str]) -> None:
 
 
 HIP_SOURCES = ["flare_hip.hip", "mvs_q8_0.hip", "mvs_q4k.hip", "mvs_f32.hip", "attn.hip", "verify.hip", "mvo.hip", "seq.hip",
-               "sample.hip", "fused.hip", "bgemm.hip", "attw.hip"]
-HOST_SOURCES = ["synth.cpp", "generate.cpp", "gguf.cpp"]
+               "sample.hip", "fused.hip", "bgemm.hip", "attw.hip", "pages.hip"]
+HOST_SOURCES = ["synth.cpp", "generate.cpp", "gguf.cpp", "pages_host.cpp"]
 
 
 def build(verbose: bool = True) -> str:

@@ -376,6 +376,7 @@ static int fail(fl_ctx *ctx, int code, const char *fmt, ...) {
 }
 
 int fl_host_fail(fl_ctx *ctx, int code, const char *msg) { return fail(ctx, code, "%s", msg); }
+int fl_ctx_device(const fl_ctx *ctx) { return ctx ? ctx->device : -1; }
 
 #define HIPCHK(ctx, expr)                                                                   \
     do {                                                                                    \

@@ -1,5 +1,5 @@
-// Internal interface between the host-only translation units (generate.cpp,
-// gguf.cpp) and the library core (flare_hip.hip).  Not part of the C-ABI.
+// Internal interface between the other translation units with entry points
+// (generate.cpp, gguf.cpp, pages.hip) and the library core (flare_hip.hip).  Not part of the C-ABI.
 #pragma once
 
 struct fl_ctx;

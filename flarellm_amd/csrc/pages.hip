@@ -1,0 +1,544 @@
+// Paged KV cache: the fl_pages_* entry points, and the launches of the kernels in
+// pages_kernels.h.
+#include <algorithm>
+#include <cmath>
+#include <cstdarg>
+#include <cstdio>
+#include <cstring>
+#include <new>
+
+#include "host_api.h"
+#include "pages_kernels.h"
+
+using namespace fl;
+
+namespace {
+
+// Pinned host memory that a copy to the device reads: written again only when that
+// copy is done.
+struct Stage {
+    char *host = nullptr;
+    size_t cap = 0;
+    hipEvent_t done = nullptr;
+    bool used = false;
+};
+constexpr int kStages = 4;
+
+struct DevBuf {
+    char *p = nullptr;
+    size_t cap = 0;
+};
+
+}  // namespace
+
+struct fl_pages {
+    fl_ctx *ctx = nullptr;  // nullptr: bookkeeping alone
+    int device = 0;
+    hipStream_t stream = nullptr;
+    fl_pages_config cfg{};
+    PagePool pool{};
+    PageTable t;
+    // the last attention call's plan: built again when its arguments or the tables change
+    PagePlan plan;
+    std::vector<int32_t> plan_seqs, plan_seen;
+    int plan_heads = 0;
+    uint64_t plan_version = 0;
+    size_t plan_items[kPageTiles] = {}, plan_order = 0, plan_pages = 0, plan_units = 0, plan_joins = 0;  // offsets
+    DevBuf d_plan, d_slots, d_read, d_copies, ws;
+    Stage stages[kStages];
+    int stage = 0;
+};
+
+namespace {
+
+int fail(fl_pages *p, int code, const char *fmt, ...) __attribute__((format(printf, 3, 4)));
+int fail(fl_pages *p, int code, const char *fmt, ...) {
+    char buf[512];
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(buf, sizeof buf, fmt, ap);
+    va_end(ap);
+    return fl_host_fail(p ? p->ctx : nullptr, code, buf);
+}
+
+#define PGCHK(p, expr)                                                                                     \
+    do {                                                                                                   \
+        const hipError_t e_ = (expr);                                                                      \
+        if (e_ != hipSuccess) return fail((p), FL_E_HIP, "%s failed: %s", #expr, hipGetErrorString(e_));   \
+    } while (0)
+#define PGTRY(expr)           \
+    do {                      \
+        const int rc_ = (expr); \
+        if (rc_) return rc_;  \
+    } while (0)
+
+// The pool's device for the length of a call, the caller's behind it.
+struct OnDevice {
+    int before = -1;
+    explicit OnDevice(const fl_pages *p) {
+        int now = 0;
+        if (p->ctx && hipGetDevice(&now) == hipSuccess && now != p->device && hipSetDevice(p->device) == hipSuccess)
+            before = now;
+    }
+    ~OnDevice() {
+        if (before >= 0) (void)hipSetDevice(before);
+    }
+};
+
+size_t elem_bytes(int fmt) { return fmt == FL_KV_F32 ? 4 : fmt == FL_KV_F16 ? 2 : 1; }
+
+int check_config(const fl_pages_config *c) {
+    if (!c) return fail(nullptr, FL_E_INVALID, "null config");
+    if (c->kv_format != FL_KV_F32 && c->kv_format != FL_KV_F16 && c->kv_format != FL_KV_Q8)
+        return fail(nullptr, FL_E_UNSUPPORTED, "paged cache of format %d", c->kv_format);
+    if (c->head_dim != 64 && c->head_dim != 128)
+        return fail(nullptr, FL_E_UNSUPPORTED, "head_dim %d (64 or 128)", c->head_dim);
+    if (c->page_size < 32 || c->page_size > 4096 || c->page_size % 32)
+        return fail(nullptr, FL_E_INVALID, "page size %d (a multiple of 32 up to 4096)", c->page_size);
+    if (c->num_layers < 1 || c->num_kv_heads < 1 || (long long)c->num_layers * c->num_kv_heads > 65535)
+        return fail(nullptr, FL_E_INVALID, "%d layers of %d kv heads", c->num_layers, c->num_kv_heads);
+    if (c->num_pages < 1 || (long long)c->num_pages * c->page_size > 0x7FFFFFFFll)
+        return fail(nullptr, FL_E_INVALID, "%d pages of %d tokens", c->num_pages, c->page_size);
+    if (c->max_seqs < 1 || c->max_seq_len < 1 || c->max_seq_len > (1 << 24) ||
+        (long long)c->max_seqs * ((c->max_seq_len + c->page_size - 1) / c->page_size) > (1ll << 28))
+        return fail(nullptr, FL_E_INVALID, "%d sequences of up to %d tokens", c->max_seqs, c->max_seq_len);
+    return 0;
+}
+
+// No call may be recorded into a graph: its replays would not move the bookkeeping.
+int check_stream(fl_pages *p) {
+    if (!p->ctx) return fail(p, FL_E_STATE, "the pages have no device memory");
+    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+    PGCHK(p, hipStreamIsCapturing(p->stream, &st));
+    if (st != hipStreamCaptureStatusNone) return fail(p, FL_E_STATE, "a paged cache's calls cannot be captured into a graph");
+    return 0;
+}
+
+// What was in a grown buffer is lost; work that reads it is done when hipFree returns.
+int ensure(fl_pages *p, DevBuf &b, size_t bytes) {
+    if (b.cap >= bytes) return 0;
+    const size_t cap = std::max(bytes, std::max<size_t>(4096, 2 * b.cap));
+    char *n = nullptr;
+    hipError_t e = hipMalloc((void **)&n, cap);
+    if (e != hipSuccess) {
+        (void)hipGetLastError();
+        return fail(p, FL_E_OOM, "hipMalloc(%zu) failed: %s", cap, hipGetErrorString(e));
+    }
+    if (b.p) {
+        (void)hipStreamSynchronize(p->stream);
+        (void)hipFree(b.p);
+    }
+    b.p = n;
+    b.cap = cap;
+    return 0;
+}
+
+// Pinned memory for `bytes` that go to the device with send().
+int stage_for(fl_pages *p, size_t bytes, char **host) {
+    Stage &s = p->stages[p->stage];
+    if (s.used) PGCHK(p, hipEventSynchronize(s.done));
+    s.used = false;
+    if (s.cap < bytes) {
+        const size_t cap = std::max<size_t>(4096, 2 * bytes);
+        char *n = nullptr;
+        if (hipHostMalloc((void **)&n, cap, hipHostMallocDefault) != hipSuccess) {
+            (void)hipGetLastError();
+            return fail(p, FL_E_OOM, "hipHostMalloc(%zu) failed", cap);
+        }
+        if (s.host) (void)hipHostFree(s.host);
+        s.host = n;
+        s.cap = cap;
+    }
+    if (!s.done) PGCHK(p, hipEventCreateWithFlags(&s.done, hipEventDisableTiming));
+    *host = s.host;
+    return 0;
+}
+
+int send(fl_pages *p, void *dev, size_t bytes) {
+    Stage &s = p->stages[p->stage];
+    PGCHK(p, hipMemcpyAsync(dev, s.host, bytes, hipMemcpyHostToDevice, p->stream));
+    PGCHK(p, hipEventRecord(s.done, p->stream));
+    s.used = true;
+    p->stage = (p->stage + 1) % kStages;
+    return 0;
+}
+
+int upload(fl_pages *p, DevBuf &b, const void *data, size_t bytes) {
+    char *h;
+    PGTRY(ensure(p, b, bytes));
+    PGTRY(stage_for(p, bytes, &h));
+    memcpy(h, data, bytes);
+    return send(p, b.p, bytes);
+}
+
+int run_copies(fl_pages *p) {
+    const auto &c = p->t.copies;
+    if (c.empty()) return 0;
+    PGTRY(upload(p, p->d_copies, c.data(), c.size() * sizeof(PageCopy)));
+    const int D = p->cfg.head_dim, unit = 32 * D * (int)elem_bytes(p->cfg.kv_format);
+    const int sunit = p->cfg.kv_format == FL_KV_Q8 ? 2 * D : 0;
+    hipLaunchKernelGGL(k_pages_copy, dim3((unsigned)c.size(), p->pool.layers * p->pool.nkv), dim3(256), 0, p->stream,
+                       p->pool, (const PageCopy *)p->d_copies.p, unit, sunit);
+    PGCHK(p, hipGetLastError());
+    return 0;
+}
+
+// Runs `op` on the bookkeeping, with its error as the context's.
+template <typename F>
+int on_table(fl_pages *p, F op) {
+    if (!p) return fail(p, FL_E_INVALID, "null pages");
+    try {
+        const int rc = op(p->t);
+        return rc ? fail(p, rc, "%s", p->t.error.c_str()) : 0;
+    } catch (const std::bad_alloc &) {
+        return fail(p, FL_E_OOM, "out of host memory");
+    } catch (...) {
+        return fail(p, FL_E_INVALID, "unexpected host error");
+    }
+}
+
+template <typename F>
+int with_form(int fmt, int D, F f) {
+    if (D == 64) return fmt == FL_KV_F32 ? f.template operator()<FL_KV_F32, 64>() :
+                        fmt == FL_KV_F16 ? f.template operator()<FL_KV_F16, 64>() : f.template operator()<FL_KV_Q8, 64>();
+    return fmt == FL_KV_F32 ? f.template operator()<FL_KV_F32, 128>() :
+           fmt == FL_KV_F16 ? f.template operator()<FL_KV_F16, 128>() : f.template operator()<FL_KV_Q8, 128>();
+}
+
+struct LaunchAttn {
+    hipStream_t st;
+    const PageAttnArgs &a;
+    int items, form;
+    template <int FMT, int D>
+    int operator()() const {
+        const dim3 grid((unsigned)(items * a.pool.nkv));
+        if (form == 0) hipLaunchKernelGGL((k_pages_attn<FMT, D, 1>), grid, dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((k_pages_attn<FMT, D, 2>), grid, dim3(256), 0, st, a);
+        return (int)hipGetLastError();
+    }
+};
+
+struct LaunchWrite {
+    hipStream_t st;
+    const PageWriteArgs &a;
+    template <int FMT, int D>
+    int operator()() const {
+        const long long total = (long long)a.layers * a.n * a.pool.nkv * (D / 32) * 2;
+        hipLaunchKernelGGL((k_pages_write<FMT, D>), dim3((unsigned)((total + 255) / 256)), dim3(256), 0, st, a);
+        return (int)hipGetLastError();
+    }
+};
+
+struct LaunchRead {
+    hipStream_t st;
+    const PageReadArgs &a;
+    template <int FMT, int D>
+    int operator()() const {
+        const long long total = (long long)a.n * a.pool.nkv * D;
+        hipLaunchKernelGGL((k_pages_read<FMT, D>), dim3((unsigned)((total + 255) / 256)), dim3(256), 0, st, a);
+        return (int)hipGetLastError();
+    }
+};
+
+// The plan of these queries, on the device.
+int make_plan(fl_pages *p, const int32_t *seqs, const int32_t *seen, int n, int heads) {
+    const int group = heads / p->cfg.num_kv_heads;
+    if (p->plan_version == p->t.version && p->plan_heads == heads && (int)p->plan_seqs.size() == n &&
+        !memcmp(p->plan_seqs.data(), seqs, n * sizeof *seqs) && !memcmp(p->plan_seen.data(), seen, n * sizeof *seen))
+        return 0;
+    p->plan_version = 0;
+    PGTRY(on_table(p, [&](PageTable &t) {
+        const int rc = page_plan(t, seqs, seen, n, group, p->cfg.num_kv_heads, p->plan);
+        if (rc) return rc;
+        p->plan_seqs.assign(seqs, seqs + n);
+        p->plan_seen.assign(seen, seen + n);
+        return 0;
+    }));
+    const PagePlan &l = p->plan;
+    size_t bytes = 0;
+    auto place = [&](size_t b) {
+        const size_t at = bytes;
+        bytes = (bytes + b + 63) / 64 * 64;
+        return at;
+    };
+    for (int f = 0; f < kPageTiles; f++) p->plan_items[f] = place(l.items[f].size() * sizeof(PageItem));
+    p->plan_order = place(l.order.size() * sizeof(PageQuery));
+    p->plan_pages = place(l.page_ids.size() * sizeof(int));
+    p->plan_units = place(l.units.size() * sizeof(int));
+    p->plan_joins = place(l.joins.size() * sizeof(PageJoin));
+    char *h;
+    PGTRY(ensure(p, p->d_plan, bytes));
+    PGTRY(ensure(p, p->ws, (size_t)l.num_units * heads * (p->cfg.head_dim + 2) * sizeof(float)));
+    PGTRY(stage_for(p, bytes, &h));
+    auto put = [&](size_t at, const auto &v) {
+        if (!v.empty()) memcpy(h + at, v.data(), v.size() * sizeof v[0]);
+    };
+    for (int f = 0; f < kPageTiles; f++) put(p->plan_items[f], l.items[f]);
+    put(p->plan_order, l.order);
+    put(p->plan_pages, l.page_ids);
+    put(p->plan_units, l.units);
+    put(p->plan_joins, l.joins);
+    PGTRY(send(p, p->d_plan.p, bytes));
+    p->plan_heads = heads;
+    p->plan_version = p->t.version;
+    return 0;
+}
+
+int check_layers(fl_pages *p, int layer, int layers) {
+    if (layer < 0 || layers < 1 || layer > p->cfg.num_layers - layers)
+        return fail(p, FL_E_INVALID, "layers %d..%d of %d", layer, layer + layers - 1, p->cfg.num_layers);
+    return 0;
+}
+
+}  // namespace
+
+int fl_pages_bytes(const fl_pages_config *cfg, size_t *kv_bytes, size_t *scale_bytes) {
+    PGTRY(check_config(cfg));
+    const size_t values = (size_t)cfg->num_layers * cfg->num_pages * cfg->num_kv_heads * cfg->page_size * cfg->head_dim;
+    if (kv_bytes) *kv_bytes = values * elem_bytes(cfg->kv_format);
+    if (scale_bytes) *scale_bytes = cfg->kv_format == FL_KV_Q8 ? values / 32 * 2 : 0;
+    return 0;
+}
+
+int fl_pages_create(fl_ctx *ctx, const fl_pages_config *cfg, void *k, void *v, void *k_scale, void *v_scale,
+                    fl_pages **out) {
+    if (!out) return fail(nullptr, FL_E_INVALID, "out is null");
+    *out = nullptr;
+    PGTRY(check_config(cfg));
+    const bool q8 = cfg->kv_format == FL_KV_Q8;
+    if (ctx) {
+        if (!k || !v || (q8 && (!k_scale || !v_scale))) return fl_host_fail(ctx, FL_E_INVALID, "null pool memory");
+        for (const void *p : {k, v, q8 ? k_scale : nullptr, q8 ? v_scale : nullptr})
+            if ((uintptr_t)p % 16) return fl_host_fail(ctx, FL_E_INVALID, "pool memory is not aligned to 16 bytes");
+    }
+    fl_pages *p = new (std::nothrow) fl_pages();
+    if (!p) return fl_host_fail(ctx, FL_E_OOM, "out of host memory");
+    p->ctx = ctx;
+    p->cfg = *cfg;
+    p->pool = PagePool{k, v, (uint16_t *)k_scale, (uint16_t *)v_scale, cfg->num_layers, cfg->num_pages, cfg->page_size,
+                       cfg->num_kv_heads};
+    if (ctx) {
+        p->device = fl_ctx_device(ctx);
+        p->stream = (hipStream_t)fl_ctx_stream(ctx);
+    }
+    int rc = on_table(p, [&](PageTable &t) { return t.init(*cfg); });
+    if (!rc && ctx) {
+        OnDevice on(p);
+        // (a call's copies go to as many pages at most, so this never fails later)
+        rc = ensure(p, p->d_copies, (size_t)cfg->num_pages * sizeof(PageCopy));
+    }
+    if (rc) {
+        fl_pages_destroy(p);
+        return rc;
+    }
+    *out = p;
+    return 0;
+}
+
+void fl_pages_destroy(fl_pages *p) {
+    if (!p) return;
+    if (p->ctx) {
+        OnDevice on(p);
+        // (hipFree waits for the device, so the context may be gone already)
+        for (DevBuf *b : {&p->d_plan, &p->d_slots, &p->d_read, &p->d_copies, &p->ws})
+            if (b->p) (void)hipFree(b->p);
+        for (Stage &s : p->stages) {
+            if (s.done) (void)hipEventDestroy(s.done);
+            if (s.host) (void)hipHostFree(s.host);
+        }
+    }
+    delete p;
+}
+
+int fl_pages_fork(fl_pages *p, const int32_t *src, const int32_t *dst, const int32_t *lens, int n) {
+    return on_table(p, [&](PageTable &t) { return t.fork(src, dst, lens, n); });
+}
+
+int fl_pages_free(fl_pages *p, const int32_t *seqs, int n) {
+    return on_table(p, [&](PageTable &t) { return t.release(seqs, n); });
+}
+
+int fl_pages_truncate(fl_pages *p, const int32_t *seqs, const int32_t *lens, int n) {
+    return on_table(p, [&](PageTable &t) { return t.truncate(seqs, lens, n); });
+}
+
+int fl_pages_copy(fl_pages *p, const int32_t *src, const int32_t *dst, int n) {
+    if (p && p->ctx) PGTRY(check_stream(p));
+    PGTRY(on_table(p, [&](PageTable &t) { return t.copy(src, dst, n); }));
+    if (!p->ctx) return 0;
+    OnDevice on(p);
+    return run_copies(p);
+}
+
+int fl_pages_compact(fl_pages *p, int *moved) {
+    if (p && p->ctx) PGTRY(check_stream(p));
+    PGTRY(on_table(p, [&](PageTable &t) { return t.compact(); }));
+    if (moved) *moved = (int)p->t.copies.size();
+    if (!p->ctx) return 0;
+    OnDevice on(p);
+    return run_copies(p);
+}
+
+int fl_pages_extend(fl_pages *p, const int32_t *seqs, const int32_t *counts, int n) {
+    if (!p) return fail(p, FL_E_INVALID, "null pages");
+    if (!p->ctx) return on_table(p, [&](PageTable &t) { return t.extend(seqs, counts, n); });
+    PGTRY(check_stream(p));
+    OnDevice on(p);
+    // room for the slots first: nothing fails behind the bookkeeping
+    long long tokens = 0;
+    for (int i = 0; i < n && counts; i++) tokens += std::min(std::max(counts[i], 0), p->cfg.max_seq_len);
+    tokens = std::min(tokens, (long long)p->cfg.num_pages * p->cfg.page_size);
+    PGTRY(ensure(p, p->d_slots, (size_t)tokens * sizeof(int)));
+    PGTRY(on_table(p, [&](PageTable &t) { return t.extend(seqs, counts, n); }));
+    if (!p->t.slots.empty()) PGTRY(upload(p, p->d_slots, p->t.slots.data(), p->t.slots.size() * sizeof(int)));
+    return run_copies(p);
+}
+
+int fl_pages_write(fl_pages *p, int layer, int layers, const float *k, const float *v, size_t row_stride) {
+    if (!p) return fail(p, FL_E_INVALID, "null pages");
+    PGTRY(check_layers(p, layer, layers));
+    PGTRY(check_stream(p));
+    const size_t row = (size_t)p->cfg.num_kv_heads * p->cfg.head_dim;
+    if (!k || !v) return fail(p, FL_E_INVALID, "null keys or values");
+    if (((uintptr_t)k | (uintptr_t)v) % 4) return fail(p, FL_E_INVALID, "keys or values are not aligned");
+    if (row_stride < row) return fail(p, FL_E_INVALID, "rows of %zu values %zu apart", row, row_stride);
+    if (!p->t.slots_valid) return fail(p, FL_E_STATE, "fl_pages_write follows fl_pages_extend, with no other change between");
+    if (p->t.slots.empty()) return 0;
+    OnDevice on(p);
+    PageWriteArgs a{};
+    a.pool = p->pool;
+    a.slots = (const int *)p->d_slots.p;
+    a.k = k;
+    a.v = v;
+    a.stride = (long long)row_stride;
+    a.layer0 = layer;
+    a.layers = layers;
+    a.n = (int)p->t.slots.size();
+    PGCHK(p, (hipError_t)with_form(p->cfg.kv_format, p->cfg.head_dim, LaunchWrite{p->stream, a}));
+    return 0;
+}
+
+int fl_pages_read(fl_pages *p, int layer, const int32_t *seqs, const int32_t *starts, const int32_t *counts, int n,
+                  float *k, float *v) {
+    if (!p) return fail(p, FL_E_INVALID, "null pages");
+    PGTRY(check_layers(p, layer, 1));
+    PGTRY(check_stream(p));
+    if (n < 0 || (n > 0 && (!seqs || !starts || !counts))) return fail(p, FL_E_INVALID, "bad sequence list");
+    std::vector<int> slots;
+    PGTRY(on_table(p, [&](PageTable &t) {
+        long long total = 0;
+        for (int i = 0; i < n; i++) {
+            if (seqs[i] < 0 || seqs[i] >= t.seqs || starts[i] < 0 || counts[i] < 0 ||
+                (long long)starts[i] + counts[i] > t.len[seqs[i]]) {
+                t.error = "tokens that are not there";
+                return FL_E_INVALID;
+            }
+            total += counts[i];
+        }
+        if (total > 0x7FFFFFFFll) {
+            t.error = "too many tokens";
+            return FL_E_INVALID;
+        }
+        slots.reserve(total);
+        for (int i = 0; i < n; i++)
+            for (int j = starts[i]; j < starts[i] + counts[i]; j++)
+                slots.push_back(t.row(seqs[i])[j / t.page_size] * t.page_size + j % t.page_size);
+        return 0;
+    }));
+    if (slots.empty()) return 0;
+    if (!k && !v) return fail(p, FL_E_INVALID, "null keys and values");
+    OnDevice on(p);
+    PGTRY(upload(p, p->d_read, slots.data(), slots.size() * sizeof(int)));
+    PageReadArgs a{p->pool, (const int *)p->d_read.p, k, v, layer, (int)slots.size()};
+    PGCHK(p, (hipError_t)with_form(p->cfg.kv_format, p->cfg.head_dim, LaunchRead{p->stream, a}));
+    return 0;
+}
+
+int fl_pages_attention(fl_pages *p, int layer, const float *q, size_t q_stride, const int32_t *seqs,
+                       const int32_t *seen, int n, int num_heads, float *out) {
+    if (!p) return fail(p, FL_E_INVALID, "null pages");
+    PGTRY(check_layers(p, layer, 1));
+    const int D = p->cfg.head_dim, nkv = p->cfg.num_kv_heads;
+    if (num_heads < 1 || num_heads % nkv) return fail(p, FL_E_INVALID, "%d heads over %d kv heads", num_heads, nkv);
+    if (num_heads / nkv > 16 * kPageTiles) return fail(p, FL_E_UNSUPPORTED, "%d query heads per kv head", num_heads / nkv);
+    if (n < 0) return fail(p, FL_E_INVALID, "%d queries", n);
+    if (n == 0) return 0;
+    if (!q || !out || !seqs || !seen) return fail(p, FL_E_INVALID, "null argument");
+    if ((uintptr_t)q % 4 || (uintptr_t)out % 16) return fail(p, FL_E_INVALID, "queries or result are not aligned");
+    if (q_stride < (size_t)num_heads * D) return fail(p, FL_E_INVALID, "queries of %d values %zu apart", num_heads * D, q_stride);
+    PGTRY(check_stream(p));
+    OnDevice on(p);
+    PGTRY(make_plan(p, seqs, seen, n, num_heads));
+    const PagePlan &l = p->plan;
+    const char *d = p->d_plan.p;
+    PageAttnArgs a{};
+    a.pool = p->pool;
+    a.layer = layer;
+    a.group = num_heads / nkv;
+    a.scale = (float)(1.4426950408889634 / std::sqrt((double)D));
+    a.q = q;
+    a.q_stride = (long long)q_stride;
+    a.order = (const PageQuery *)(d + p->plan_order);
+    a.page_ids = (const int *)(d + p->plan_pages);
+    a.part = (float *)p->ws.p;
+    a.ml = a.part + (size_t)l.num_units * num_heads * D;
+    a.out = out;
+    for (int f = kPageTiles - 1; f >= 0; f--) {
+        if (l.items[f].empty()) continue;
+        a.items = (const PageItem *)(d + p->plan_items[f]);
+        PGCHK(p, (hipError_t)with_form(p->cfg.kv_format, D, LaunchAttn{p->stream, a, (int)l.items[f].size(), f}));
+    }
+    if (!l.joins.empty()) {
+        PageJoinArgs j{(const PageJoin *)(d + p->plan_joins), (const int *)(d + p->plan_units), a.part, a.ml, out, num_heads};
+        const dim3 grid((unsigned)l.joins.size(), (unsigned)((num_heads * D + 1023) / 1024));
+        if (D == 64) hipLaunchKernelGGL(k_pages_join<64>, grid, dim3(256), 0, p->stream, j);
+        else hipLaunchKernelGGL(k_pages_join<128>, grid, dim3(256), 0, p->stream, j);
+        PGCHK(p, hipGetLastError());
+    }
+    return 0;
+}
+
+int fl_pages_len(const fl_pages *p, int seq) { return p && seq >= 0 && seq < p->t.seqs ? p->t.len[seq] : -1; }
+
+int fl_pages_free_count(const fl_pages *p) { return p ? p->t.free_pages : -1; }
+
+int fl_pages_tables(const fl_pages *p, int32_t *tables, int32_t *lens) {
+    if (!p) return fl_host_fail(nullptr, FL_E_INVALID, "null pages");
+    if (tables) memcpy(tables, p->t.table.data(), p->t.table.size() * sizeof(int));
+    if (lens) memcpy(lens, p->t.len.data(), p->t.len.size() * sizeof(int));
+    return 0;
+}
+
+int fl_pages_copies(const fl_pages *p, int32_t *copies, int cap) {
+    if (!p) return -1;
+    const auto &c = p->t.copies;
+    for (int i = 0; copies && i < cap && i < (int)c.size(); i++) {
+        copies[3 * i] = c[i].src;
+        copies[3 * i + 1] = c[i].dst;
+        copies[3 * i + 2] = c[i].blocks;
+    }
+    return (int)c.size();
+}
+
+int fl_pages_plan(fl_pages *p, const int32_t *seqs, const int32_t *seen, int n, int num_heads, int32_t *items, int cap) {
+    if (!p) return fail(p, FL_E_INVALID, "null pages");
+    const int nkv = p->cfg.num_kv_heads;
+    if (num_heads < 1 || num_heads % nkv || num_heads / nkv > 16 * kPageTiles)
+        return fail(p, FL_E_INVALID, "%d heads over %d kv heads", num_heads, nkv);
+    int made = 0;
+    PGTRY(on_table(p, [&](PageTable &t) {
+        PagePlan l;
+        const int rc = page_plan(t, seqs, seen, n, num_heads / nkv, nkv, l);
+        if (rc) return rc;
+        for (int f = 0; f < kPageTiles; f++)
+            for (const PageItem &it : l.items[f])
+                for (int i = 0; i < it.nq; i++, made++) {
+                    if (!items || made >= cap) continue;
+                    const int row[6] = {l.order[it.q0 + i].query, it.slot0, it.slot1, l.page_ids[it.page0], f,
+                                        it.unit < 0 ? -1 : it.unit + i};
+                    memcpy(items + 6 * made, row, sizeof row);
+                }
+        return 0;
+    }));
+    return made;
+}

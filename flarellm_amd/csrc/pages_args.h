@@ -1,0 +1,55 @@
+// Arguments of the paged-cache kernels (pages_kernels.h, included by pages.hip only).
+#pragma once
+
+#include "kernels.h"
+#include "pages_host.h"
+
+namespace fl {
+
+// The pool: K [layer][page][kv head][slot][D], V [layer][page][kv head][slot / 32][D][32]
+// (f32, binary16, or int8 codes with a binary16 scale per 32 channels, [layer][page]
+// [kv head][slot][D / 32] for each).  A (page, kv head) of either begins at the same
+// element: ((layer * pages + page) * nkv + head) * P * D.
+struct PagePool {
+    void *k, *v;
+    uint16_t *ks, *vs;  // Q8
+    int layers, pages, P, nkv;
+};
+
+struct PageAttnArgs {
+    PagePool pool;
+    int layer, group;
+    float scale;           // log2(e) / sqrt(D)
+    const float *q;        // query i, head h at i * q_stride + h * D
+    long long q_stride;
+    const PageItem *items;
+    const PageQuery *order;
+    const int *page_ids;
+    float *part, *ml;      // partial results [unit][head][D], [unit][head][2] = (max, sum)
+    float *out;            // [n][heads * D]
+};
+
+struct PageJoinArgs {
+    const PageJoin *joins;
+    const int *units;
+    const float *part, *ml;
+    float *out;
+    int heads;
+};
+
+struct PageWriteArgs {
+    PagePool pool;
+    const int *slots;      // page * P + slot of each token
+    const float *k, *v;    // token i, kv head h at (layer * n + i) * stride + h * D
+    long long stride;
+    int layer0, layers, n;
+};
+
+struct PageReadArgs {
+    PagePool pool;
+    const int *slots;
+    float *k, *v;          // [n][nkv * D]
+    int layer, n;
+};
+
+}  // namespace fl

@@ -1,0 +1,390 @@
+// Page bookkeeping and attention plans of the paged KV cache (pages_host.h).
+#include "pages_host.h"
+
+#include <algorithm>
+#include <climits>
+#include <cstdarg>
+#include <cstdio>
+#include <numeric>
+
+namespace fl {
+
+namespace {
+int ceil_div(int a, int b) { return (int)(((long long)a + b - 1) / b); }
+}  // namespace
+
+int PageTable::fail(int code, const char *fmt, ...) {
+    char buf[256];
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(buf, sizeof buf, fmt, ap);
+    va_end(ap);
+    error = buf;
+    return code;
+}
+
+int PageTable::init(const fl_pages_config &c) {
+    pages = c.num_pages;
+    page_size = c.page_size;
+    seqs = c.max_seqs;
+    max_len = c.max_seq_len;
+    max_pages = ceil_div(max_len, page_size);
+    free_pages = pages;
+    table.assign((size_t)seqs * max_pages, -1);
+    len.assign(seqs, 0);
+    ref.assign(pages, 0);
+    stamp.assign(std::max(seqs, pages), 0);
+    free_bits.assign((pages + 63) / 64, ~0ull);
+    if (pages % 64) free_bits.back() = (1ull << (pages % 64)) - 1;
+    return 0;
+}
+
+// The free page of lowest index (the caller has counted that there is one).
+int PageTable::take() {
+    while (!free_bits[hint]) hint++;
+    const int g = 64 * hint + __builtin_ctzll(free_bits[hint]);
+    free_bits[hint] &= free_bits[hint] - 1;
+    free_pages--;
+    ref[g] = 1;
+    return g;
+}
+
+void PageTable::drop(int g) {
+    if (--ref[g]) return;
+    free_bits[g / 64] |= 1ull << (g % 64);
+    hint = std::min(hint, g / 64);
+    free_pages++;
+}
+
+int PageTable::check_seqs(const int32_t *s, int n, bool once) {
+    if (n < 0 || (n > 0 && !s)) return fail(FL_E_INVALID, "bad sequence list");
+    stamp_now++;
+    for (int i = 0; i < n; i++) {
+        if (s[i] < 0 || s[i] >= seqs) return fail(FL_E_INVALID, "sequence %d of %d", s[i], seqs);
+        if (once && stamp[s[i]] == stamp_now) return fail(FL_E_INVALID, "sequence %d is listed twice", s[i]);
+        stamp[s[i]] = stamp_now;
+    }
+    return 0;
+}
+
+// 32-slot blocks in use of the i-th page of sequence s.
+int PageTable::blocks_of(int s, int i) const {
+    return ceil_div(std::min(page_size, len[s] - i * page_size), kPageBlock);
+}
+
+int PageTable::fork(const int32_t *src, const int32_t *dst, const int32_t *lens, int n) {
+    if (int rc = check_seqs(src, n, false)) return rc;
+    if (int rc = check_seqs(dst, n, true)) return rc;
+    for (int i = 0; i < n; i++) {
+        if (len[dst[i]]) return fail(FL_E_STATE, "sequence %d is not empty", dst[i]);
+        if (stamp[src[i]] == stamp_now) return fail(FL_E_INVALID, "sequence %d is both source and target", src[i]);
+        if (lens && (lens[i] < 0 || lens[i] > len[src[i]]))
+            return fail(FL_E_INVALID, "%d of the %d tokens of sequence %d", lens[i], len[src[i]], src[i]);
+    }
+    copies.clear();
+    for (int i = 0; i < n; i++) {
+        len[dst[i]] = lens ? lens[i] : len[src[i]];
+        const int m = held(dst[i]), *from = row(src[i]);
+        std::copy(from, from + m, row(dst[i]));
+        for (int j = 0; j < m; j++) ref[from[j]]++;
+    }
+    slots_valid = false;
+    version++;
+    return 0;
+}
+
+int PageTable::copy(const int32_t *src, const int32_t *dst, int n) {
+    if (int rc = check_seqs(src, n, false)) return rc;
+    if (int rc = check_seqs(dst, n, true)) return rc;
+    long long need = 0;
+    for (int i = 0; i < n; i++) {
+        if (len[dst[i]]) return fail(FL_E_STATE, "sequence %d is not empty", dst[i]);
+        if (stamp[src[i]] == stamp_now) return fail(FL_E_INVALID, "sequence %d is both source and target", src[i]);
+        need += held(src[i]);
+    }
+    if (need > free_pages) return fail(FL_E_OOM, "%lld pages needed, %d free", need, free_pages);
+    copies.clear();
+    copies.reserve(need);
+    for (int i = 0; i < n; i++) {
+        const int m = held(src[i]);
+        len[dst[i]] = len[src[i]];
+        for (int j = 0; j < m; j++) {
+            const int g = row(dst[i])[j] = take();
+            copies.push_back({row(src[i])[j], g, blocks_of(src[i], j)});
+        }
+    }
+    slots_valid = false;
+    version++;
+    return 0;
+}
+
+int PageTable::release(const int32_t *s, int n) {
+    if (int rc = check_seqs(s, n, false)) return rc;
+    copies.clear();
+    for (int i = 0; i < n; i++) {
+        int *r = row(s[i]);
+        for (int j = 0, m = held(s[i]); j < m; j++) {
+            drop(r[j]);
+            r[j] = -1;
+        }
+        len[s[i]] = 0;
+    }
+    slots_valid = false;
+    version++;
+    return 0;
+}
+
+int PageTable::truncate(const int32_t *s, const int32_t *lens, int n) {
+    if (int rc = check_seqs(s, n, true)) return rc;
+    if (n > 0 && !lens) return fail(FL_E_INVALID, "no lengths");
+    for (int i = 0; i < n; i++)
+        if (lens[i] < 0 || lens[i] > len[s[i]])
+            return fail(FL_E_INVALID, "%d of the %d tokens of sequence %d", lens[i], len[s[i]], s[i]);
+    copies.clear();
+    for (int i = 0; i < n; i++) {
+        int *r = row(s[i]);
+        const int m = held(s[i]);
+        len[s[i]] = lens[i];
+        for (int j = held(s[i]); j < m; j++) {
+            drop(r[j]);
+            r[j] = -1;
+        }
+    }
+    slots_valid = false;
+    version++;
+    return 0;
+}
+
+int PageTable::extend(const int32_t *s, const int32_t *counts, int n) {
+    if (int rc = check_seqs(s, n, true)) return rc;
+    if (n > 0 && !counts) return fail(FL_E_INVALID, "no counts");
+    long long tokens = 0, need = 0;
+    for (int i = 0; i < n; i++) {
+        if (counts[i] < 0) return fail(FL_E_INVALID, "%d new tokens", counts[i]);
+        if (counts[i] > max_len - len[s[i]])
+            return fail(FL_E_INVALID, "sequence %d of %d tokens cannot take %d more: at most %d", s[i], len[s[i]],
+                        counts[i], max_len);
+        tokens += counts[i];
+    }
+    // A last page that others hold too is left to them.  Where several of the
+    // call's sequences share one, all but the last of those that hold it take a copy.
+    std::vector<int> left;  // pages that the call has left, once per sequence
+    for (int i = 0; i < n; i++) {
+        need += ceil_div(len[s[i]] + counts[i], page_size) - held(s[i]);
+        if (!counts[i] || len[s[i]] % page_size == 0) continue;
+        left.push_back(row(s[i])[held(s[i]) - 1]);
+    }
+    std::sort(left.begin(), left.end());
+    for (size_t i = 0; i < left.size();) {
+        size_t j = i;
+        while (j < left.size() && left[j] == left[i]) j++;
+        need += std::min<long long>(j - i, ref[left[i]] - 1);
+        i = j;
+    }
+    if (need > free_pages) return fail(FL_E_OOM, "%lld pages needed, %d free", need, free_pages);
+    std::vector<int> out;
+    out.reserve(tokens);
+    copies.clear();
+    copies.reserve(left.size());
+    slots.swap(out);
+    for (int i = 0; i < n; i++) {
+        int *r = row(s[i]), at = len[s[i]];
+        const int last = held(s[i]) - 1;
+        if (counts[i] && at % page_size && ref[r[last]] > 1) {
+            const int g = take();
+            copies.push_back({r[last], g, blocks_of(s[i], last)});
+            ref[r[last]]--;
+            r[last] = g;
+        }
+        len[s[i]] += counts[i];
+        for (int j = last + 1; j < held(s[i]); j++) r[j] = take();
+        for (; at < len[s[i]]; at++) slots.push_back(r[at / page_size] * page_size + at % page_size);
+    }
+    slots_valid = true;
+    version++;
+    return 0;
+}
+
+int PageTable::compact() {
+    const int used = pages - free_pages;
+    // pages at or above `used` in use, and free ones below: equally many
+    std::vector<int> to(pages, -1), fill(pages, 0);
+    std::vector<PageCopy> moves;
+    for (int g = used, d = 0; g < pages; g++) {
+        if (!ref[g]) continue;
+        while (ref[d]) d++;
+        to[g] = d;
+        moves.push_back({g, d++, 0});
+    }
+    for (int s = 0; s < seqs; s++)
+        for (int j = 0, m = held(s); j < m; j++) fill[row(s)[j]] = std::max(fill[row(s)[j]], blocks_of(s, j));
+    copies.clear();
+    slots_valid = false;
+    if (moves.empty()) return 0;
+    for (PageCopy &c : moves) {
+        c.blocks = fill[c.src];
+        std::swap(ref[c.src], ref[c.dst]);
+        free_bits[c.src / 64] |= 1ull << (c.src % 64);
+        free_bits[c.dst / 64] &= ~(1ull << (c.dst % 64));
+    }
+    copies.swap(moves);
+    hint = used / 64 < (int)free_bits.size() ? used / 64 : 0;
+    for (int s = 0; s < seqs; s++)
+        for (int j = 0, m = held(s); j < m; j++)
+            if (to[row(s)[j]] >= 0) row(s)[j] = to[row(s)[j]];
+    version++;
+    return 0;
+}
+
+// ---------------------------------------------------------------------------
+// Attention plan.  The sequences of the call are sorted by their page lists, so
+// those that share leading pages are neighbours.  A run is a range of pages that
+// the same sequences hold, as long as it can be: it ends where two of them
+// differ, not where one of them ends (its queries are masked there).  So each page
+// is in one run per set of sequences that hold it, and is read once for all of
+// them.  A run's queries, longest first, are cut into tiles of up to 32 rows (query
+// x head of a kv head) and its tokens into parts, until the chip is full.
+// ---------------------------------------------------------------------------
+int page_plan(PageTable &t, const int32_t *s, const int32_t *seen, int n, int group, int kv_heads, PagePlan &p) {
+    auto fail = [&](int code, const std::string &m) {
+        t.error = m;
+        return code;
+    };
+    if (n < 0 || (n > 0 && (!s || !seen))) return fail(FL_E_INVALID, "bad query list");
+    for (int i = 0; i < n; i++) {
+        if (s[i] < 0 || s[i] >= t.seqs)
+            return fail(FL_E_INVALID, "query " + std::to_string(i) + ": sequence " + std::to_string(s[i]));
+        if (seen[i] < 0 || seen[i] > t.len[s[i]])
+            return fail(FL_E_INVALID, "query " + std::to_string(i) + " sees " + std::to_string(seen[i]) + " of " +
+                                          std::to_string(t.len[s[i]]) + " tokens");
+    }
+    for (auto &v : p.items) v.clear();
+    p.order.clear();
+    p.page_ids.clear();
+    p.units.clear();
+    p.joins.clear();
+    p.num_units = 0;
+    const int P = t.page_size;
+
+    // the call's sequences, each with its queries (longest first) and pages in view
+    struct Seq {
+        const int *pages;
+        int held;         // pages that its longest query sees
+        int first, count; // queries
+    };
+    std::vector<int> by(n);
+    std::iota(by.begin(), by.end(), 0);
+    std::stable_sort(by.begin(), by.end(), [&](int a, int b) { return s[a] != s[b] ? s[a] < s[b] : seen[a] > seen[b]; });
+    std::vector<Seq> seqs;
+    for (int i = 0; i < n; i++) {
+        if (i && s[by[i]] == s[by[i - 1]]) {
+            seqs.back().count++;
+        } else {
+            seqs.push_back({t.row(s[by[i]]), ceil_div(seen[by[i]], P), i, 1});
+        }
+    }
+    // a list that ends is behind those that go on
+    std::sort(seqs.begin(), seqs.end(), [](const Seq &a, const Seq &b) {
+        const int m = std::min(a.held, b.held);
+        const int k = (int)(std::mismatch(a.pages, a.pages + m, b.pages).first - a.pages);
+        if (k < m) return a.pages[k] < b.pages[k];
+        return a.held != b.held ? a.held > b.held : a.first < b.first;
+    });
+
+    struct Run {
+        int lo, hi, p0, p1;  // sequences, pages
+    };
+    struct Tile {
+        int q0, nq, slot0, slot1, page0, form;
+    };
+    std::vector<Run> todo{{0, (int)seqs.size(), 0, 0}};
+    std::vector<Tile> tiles;
+    const int most = std::max(1, 16 * kPageTiles / group);  // queries of the largest tile
+    while (!todo.empty()) {
+        Run r = todo.back();
+        todo.pop_back();
+        int lo = r.lo, hi = r.hi, e = r.p0;
+        for (;;) {
+            while (hi > lo && seqs[hi - 1].held <= e) hi--;  // those that have ended
+            if (lo == hi) break;
+            const Seq &a = seqs[lo], &b = seqs[hi - 1];
+            const int m = std::min(a.held, b.held);
+            const int k = (int)(std::mismatch(a.pages + e, a.pages + m, b.pages + e).first - a.pages);
+            if (k == e) break;  // they differ here
+            e = k;
+        }
+        // [lo, hi): go on behind the run, by their next page
+        for (int i = lo; i < hi;) {
+            int j = i;
+            while (j < hi && seqs[j].pages[e] == seqs[i].pages[e]) j++;
+            todo.push_back({i, j, e, 0});
+            i = j;
+        }
+        if (e == r.p0) continue;
+        const int from = r.p0 * P, first = (int)p.order.size();
+        for (int i = r.lo; i < r.hi; i++)
+            for (int j = 0; j < seqs[i].count; j++) {
+                const int q = by[seqs[i].first + j];
+                if (seen[q] <= from) break;
+                p.order.push_back({q, seen[q]});
+            }
+        const int end = e * P, total = (int)p.order.size() - first;
+        std::stable_sort(p.order.begin() + first, p.order.end(), [&](const PageQuery &a, const PageQuery &b) {
+            return std::min(a.seen, end) > std::min(b.seen, end);
+        });
+        const int page0 = (int)p.page_ids.size();
+        for (int i = r.p0; i < e; i++) p.page_ids.push_back(seqs[r.lo].pages[i]);
+        for (int i = 0; i < total; i += most) {
+            const int nq = std::min(most, total - i);
+            tiles.push_back({first + i, nq, from, std::min(p.order[first + i].seen, end), page0,
+                             std::min(kPageTiles, ceil_div(nq * group, 16)) - 1});
+        }
+    }
+
+    // Parts: about kPageFill workgroups, none of less than kPageLeast blocks
+    constexpr int kPageFill = 768, kPageLeast = 8;
+    long long blocks = 0;
+    for (const Tile &x : tiles) blocks += ceil_div(x.slot1 - x.slot0, kPageBlock);
+    const int part = (int)std::max<long long>(kPageLeast, (blocks * kv_heads + kPageFill - 1) / kPageFill);
+    std::vector<int> count(n, 0);
+    std::vector<std::pair<int, int>> at;  // form and index of every item
+    for (const Tile &x : tiles) {
+        const int nb = ceil_div(x.slot1 - x.slot0, kPageBlock), cuts = ceil_div(nb, part), each = ceil_div(nb, cuts);
+        for (int b = 0; b < nb; b += each) {
+            PageItem it{};
+            it.q0 = x.q0;
+            it.slot0 = x.slot0 + b * kPageBlock;
+            it.slot1 = std::min(x.slot1, it.slot0 + each * kPageBlock);
+            it.page0 = x.page0 + it.slot0 / P - x.slot0 / P;
+            while (it.nq < x.nq && p.order[x.q0 + it.nq].seen > it.slot0) it.nq++;
+            it.smin = p.order[x.q0 + it.nq - 1].seen;
+            for (int i = 0; i < it.nq; i++) count[p.order[x.q0 + i].query]++;
+            at.push_back({x.form, (int)p.items[x.form].size()});
+            p.items[x.form].push_back(it);
+        }
+    }
+    std::vector<int> first(n + 1, 0);
+    std::vector<char> joined(n, 0);
+    for (auto &a : at) {
+        PageItem &it = p.items[a.first][a.second];
+        bool alone = true;
+        for (int i = 0; i < it.nq; i++) alone = alone && count[p.order[it.q0 + i].query] == 1;
+        it.unit = alone ? -1 : p.num_units;
+        if (alone) continue;
+        for (int i = 0; i < it.nq; i++) joined[p.order[it.q0 + i].query] = 1;
+        p.num_units += it.nq;
+    }
+    for (int i = 0; i < n; i++) first[i + 1] = first[i] + (joined[i] ? count[i] : 0);
+    p.units.resize(first[n]);
+    for (int i = 0; i < n; i++)
+        if (joined[i] || !count[i]) p.joins.push_back({i, first[i], joined[i] ? count[i] : 0, 0});
+    std::vector<int> next(first.begin(), first.end() - 1);
+    for (auto &a : at) {
+        const PageItem &it = p.items[a.first][a.second];
+        if (it.unit < 0) continue;
+        for (int i = 0; i < it.nq; i++) p.units[next[p.order[it.q0 + i].query]++] = it.unit + i;
+    }
+    return 0;
+}
+
+}  // namespace fl

@@ -1,0 +1,94 @@
+// Host side of the paged KV cache: which sequence holds which page, and the
+// plan of an attention call.  Plain C++ without a device.
+#pragma once
+
+#include <cstdint>
+#include <string>
+#include <vector>
+
+#include "../../include/flare_hip.h"
+
+namespace fl {
+
+constexpr int kPageBlock = 32;  // slots of a block: the unit of copies and of the attention's tiles
+
+// Copy the first `blocks` 32-slot blocks of page src to page dst, in every layer.
+struct PageCopy {
+    int src, dst, blocks;
+};
+
+// Pages, their reference counts and the sequences' page lists.  Every call
+// checks its arguments before it changes anything: a call that fails leaves the
+// state as it was.
+struct PageTable {
+    int pages = 0, page_size = 0, seqs = 0, max_len = 0, max_pages = 0;
+    int free_pages = 0;
+    std::vector<int> table;  // [seqs][max_pages], -1 where a sequence holds none
+    std::vector<int> len;    // tokens of each sequence
+    std::vector<int> ref;    // sequences that hold a page
+    std::vector<PageCopy> copies;  // of the last call
+    std::vector<int> slots;        // page * page_size + slot of every token of the last extend
+    bool slots_valid = false;      // no other call since
+    uint64_t version = 1;          // changes with the tables and lengths
+    std::string error;
+
+    int init(const fl_pages_config &c);
+    int fork(const int32_t *src, const int32_t *dst, const int32_t *lens, int n);
+    int copy(const int32_t *src, const int32_t *dst, int n);
+    int release(const int32_t *s, int n);
+    int truncate(const int32_t *s, const int32_t *lens, int n);
+    int extend(const int32_t *s, const int32_t *counts, int n);
+    int compact();
+
+    int held(int s) const { return (len[s] + page_size - 1) / page_size; }
+    int *row(int s) { return table.data() + (size_t)s * max_pages; }
+    const int *row(int s) const { return table.data() + (size_t)s * max_pages; }
+
+private:
+    std::vector<uint64_t> free_bits;
+    int hint = 0;            // no free page below 64 * hint
+    std::vector<int> stamp;  // marks of one call
+    int stamp_now = 0;
+    int take();
+    void drop(int page);
+    int fail(int code, const char *fmt, ...) __attribute__((format(printf, 3, 4)));
+    int check_seqs(const int32_t *s, int n, bool once);
+    int blocks_of(int s, int i) const;
+};
+
+// One workgroup's part of an attention call, per kv head: queries order[q0 ..
+// q0 + nq) over tokens [slot0, slot1) of the sequences that share the pages
+// page_ids[page0 ..) there (the page of slot0 first).
+struct PageItem {
+    int q0, nq, slot0, slot1, page0;
+    int unit;  // partial result of the first query; -1: the item is all that its queries see
+    int smin;  // fewest tokens that one of the queries sees
+    int pad;
+};
+
+// A query in an item's order: its number, and how many tokens it sees.
+struct PageQuery {
+    int query, seen;
+};
+
+// A query whose result is joined from the partial results units[first .. first
+// + count); of none: zeros.
+struct PageJoin {
+    int query, first, count, pad;
+};
+
+constexpr int kPageTiles = 2;  // item forms: up to 16 and up to 32 rows (query x head of a kv head)
+
+struct PagePlan {
+    std::vector<PageItem> items[kPageTiles];
+    std::vector<PageQuery> order;
+    std::vector<int> page_ids, units;
+    std::vector<PageJoin> joins;
+    int num_units = 0;
+};
+
+// seen[i] tokens of sequence s[i] for query i (checked against the table).
+// group: query heads per kv head.  0, or a code and table.error.
+int page_plan(PageTable &t, const int32_t *s, const int32_t *seen, int n, int group, int kv_heads, PagePlan &p);
+
+}  // namespace fl

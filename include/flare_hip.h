@@ -102,6 +102,8 @@ const char *fl_last_error(const fl_ctx *ctx);
 /* The hipStream_t all work of this context is enqueued on. */
 void *fl_ctx_stream(fl_ctx *ctx);
 int fl_sync(fl_ctx *ctx);
+/* The HIP device of a context. */
+int fl_ctx_device(const fl_ctx *ctx);
 /* ComputeBackend::name (model.rs:615). */
 const char *fl_backend_name(void);
 
@@ -363,6 +365,90 @@ int fl_decode_continue(fl_ctx *ctx, int n_steps);
 /* Copy tokens[start, start+n) of the device token buffer (prompt tokens
  * followed by generated tokens) to the host. */
 int fl_read_tokens(fl_ctx *ctx, int start, int n, uint32_t *out);
+
+/* ---- paged KV cache of many sequences -------------------------------------- */
+/* A pool of pages of K and V rows, and sequences that are lists of pages, so that
+ * sequences share what they have in common: the answers to one prompt, the chats
+ * behind one system prompt, beams.  No counterpart in the reference, whose caches
+ * hold one sequence (kv_cache.rs:431-546); rows, formats and the attention are those
+ * of fl_kv_write and fl_gqa_from_cache, per sequence.
+ *
+ * Token j of a sequence with the pages t[] is in slot j % page_size of page
+ * t[j / page_size].  The pool's device memory is the caller's (16-byte aligned,
+ * fl_pages_bytes):
+ *   k [layer][page][kv head][slot][head_dim]
+ *   v [layer][page][kv head][slot / 32][head_dim][32]
+ * f32, binary16, or int8 codes with a binary16 scale per 32 channels:
+ *   k_scale, v_scale [layer][page][kv head][slot][head_dim / 32]   (FL_KV_Q8)
+ *
+ * The bookkeeping is the host's and immediate.  Every call checks its arguments
+ * before it changes anything, and one that fails leaves the pool and the sequences
+ * as they were (after FL_E_HIP nothing is certain).  What a call does on the device
+ * is enqueued on the context's stream, and no call waits for it; none can be
+ * captured into a graph (FL_E_STATE).  Destroy a pool before its context.  As a
+ * context, a pool is not thread-safe. */
+typedef struct fl_pages fl_pages;
+typedef struct {
+    int num_layers, num_kv_heads, head_dim; /* head_dim 64 or 128 */
+    int kv_format;                          /* FL_KV_F32, FL_KV_F16 or FL_KV_Q8 */
+    int num_pages, page_size;               /* page_size a multiple of 32, up to 4096 */
+    int max_seqs, max_seq_len;              /* sequences 0..max_seqs-1 of up to max_seq_len tokens */
+} fl_pages_config;
+/* Bytes of k (and of v), and of k_scale (and of v_scale; 0 without scales). */
+int fl_pages_bytes(const fl_pages_config *cfg, size_t *kv_bytes, size_t *scale_bytes);
+/* A pool with every page free and every sequence empty.  ctx NULL (testing
+ * surface): bookkeeping without a device, memory pointers unused. */
+int fl_pages_create(fl_ctx *ctx, const fl_pages_config *cfg, void *k, void *v, void *k_scale, void *v_scale,
+                    fl_pages **out);
+void fl_pages_destroy(fl_pages *p);
+/* Sequence dst[i] (empty before, listed once) becomes the first lens[i] tokens of
+ * src[i] (lens NULL: all of them), on the same pages: no row is copied. */
+int fl_pages_fork(fl_pages *p, const int32_t *src, const int32_t *dst, const int32_t *lens, int n);
+/* The same with pages of its own: dst[i] (empty before, listed once) gets a copy of
+ * src[i].  FL_E_OOM: not enough free pages.  Copies take the slots in use, in whole
+ * 32-slot blocks. */
+int fl_pages_copy(fl_pages *p, const int32_t *src, const int32_t *dst, int n);
+/* Empties the sequences; a page that no sequence holds any more is free. */
+int fl_pages_free(fl_pages *p, const int32_t *seqs, int n);
+/* Cuts each sequence (listed once) to its first lens[i] tokens. */
+int fl_pages_truncate(fl_pages *p, const int32_t *seqs, const int32_t *lens, int n);
+/* Reserves slots for counts[i] more tokens of each sequence (listed once), in the
+ * order of the list; a new page is the free one of lowest index.  Where a sequence
+ * would write to a page that others hold too, it first gets a copy of that page.
+ * FL_E_OOM: not enough free pages. */
+int fl_pages_extend(fl_pages *p, const int32_t *seqs, const int32_t *counts, int n);
+/* Stores keys and values of the last fl_pages_extend's tokens, sequence by sequence
+ * in its order, in `layers` layers from `layer` on: device f32, token i of the l-th
+ * of them at (l * tokens + i) * row_stride, num_kv_heads * head_dim values.  (The
+ * other calls that change sequences end this: FL_E_STATE.) */
+int fl_pages_write(fl_pages *p, int layer, int layers, const float *k, const float *v, size_t row_stride);
+/* Moves pages so that those in use are the ones of lowest index; *moved (may be
+ * NULL): how many were moved. */
+int fl_pages_compact(fl_pages *p, int *moved);
+/* The values of tokens starts[i] .. starts[i] + counts[i] - 1 of each sequence in
+ * one layer, as f32 rows [tokens][num_kv_heads * head_dim] on the device (k or v
+ * may be NULL). */
+int fl_pages_read(fl_pages *p, int layer, const int32_t *seqs, const int32_t *starts, const int32_t *counts, int n,
+                  float *k, float *v);
+/* Attention of n queries (device f32, RoPE applied, query i at q + i * q_stride,
+ * num_heads * head_dim values) over one layer: query i sees the first seen[i] tokens
+ * of sequence seqs[i] (host arrays; a sequence may have any number of queries), each
+ * as grouped_query_attention_from_gpu_cache (model.rs:311).  seen[i] = 0 gives zeros.
+ * A page that several of the call's sequences hold is read once for all of them.  out
+ * [n][num_heads * head_dim] f32, 16-byte aligned.  Up to 32 query heads per kv head. */
+int fl_pages_attention(fl_pages *p, int layer, const float *q, size_t q_stride, const int32_t *seqs,
+                       const int32_t *seen, int n, int num_heads, float *out);
+/* Tokens of a sequence, free pages of the pool (-1: no such). */
+int fl_pages_len(const fl_pages *p, int seq);
+int fl_pages_free_count(const fl_pages *p);
+/* All page lists [max_seqs][max_seq_len / page_size rounded up] (-1 where a
+ * sequence holds none) and all lengths (either may be NULL). */
+int fl_pages_tables(const fl_pages *p, int32_t *tables, int32_t *lens);
+/* Testing surface: the copies of the last call as (source page, target page, 32-slot
+ * blocks), and an attention call's plan as rows (query, first token, end, page of the
+ * first token, form, partial result or -1).  Both return the count (negative: error). */
+int fl_pages_copies(const fl_pages *p, int32_t *copies, int cap);
+int fl_pages_plan(fl_pages *p, const int32_t *seqs, const int32_t *seen, int n, int num_heads, int32_t *items, int cap);
 
 /* ---- sampling (flare-core/src/sampling.rs) ------------------------------------ */
 /* SamplingParams (sampling.rs:19-54) without the self-speculation fields
