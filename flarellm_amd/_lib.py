@@ -191,6 +191,7 @@ SIGNATURES = {
     "fl_pages_read": (i32, [vp, i32, vp, vp, vp, i32, vp, vp]),
     "fl_pages_attention": (i32, [vp, i32, vp, sz, vp, vp, i32, i32, vp]),
     "fl_pages_len": (i32, [vp, i32]),
+    "fl_pages_pending": (i32, [vp]),
     "fl_pages_free_count": (i32, [vp]),
     "fl_pages_tables": (i32, [vp, vp, vp]),
     "fl_pages_copies": (i32, [vp, vp, i32]),

@@ -43,7 +43,7 @@ struct fl_pages {
     std::vector<int32_t> plan_seqs, plan_seen;
     int plan_heads = 0;
     uint64_t plan_version = 0;
-    size_t plan_items[kPageTiles] = {}, plan_order = 0, plan_pages = 0, plan_units = 0, plan_joins = 0;  // offsets
+    size_t plan_items[kPageForms] = {}, plan_order = 0, plan_pages = 0, plan_units = 0, plan_joins = 0;  // offsets
     DevBuf d_plan, d_slots, d_read, d_copies, ws;
     Stage stages[kStages];
     int stage = 0;
@@ -174,11 +174,18 @@ int upload(fl_pages *p, DevBuf &b, const void *data, size_t bytes) {
 int run_copies(fl_pages *p) {
     const auto &c = p->t.copies;
     if (c.empty()) return 0;
-    PGTRY(upload(p, p->d_copies, c.data(), c.size() * sizeof(PageCopy)));
+    PageCopies list;
+    list.list = nullptr;
+    if (c.size() <= kInlineCopies) {
+        memcpy(list.some, c.data(), c.size() * sizeof(PageCopy));
+    } else {
+        PGTRY(upload(p, p->d_copies, c.data(), c.size() * sizeof(PageCopy)));
+        list.list = (const PageCopy *)p->d_copies.p;
+    }
     const int D = p->cfg.head_dim, unit = 32 * D * (int)elem_bytes(p->cfg.kv_format);
     const int sunit = p->cfg.kv_format == FL_KV_Q8 ? 2 * D : 0;
     hipLaunchKernelGGL(k_pages_copy, dim3((unsigned)c.size(), p->pool.layers * p->pool.nkv), dim3(256), 0, p->stream,
-                       p->pool, (const PageCopy *)p->d_copies.p, unit, sunit);
+                       p->pool, list, unit, sunit);
     PGCHK(p, hipGetLastError());
     return 0;
 }
@@ -213,7 +220,13 @@ struct LaunchAttn {
     int operator()() const {
         const dim3 grid((unsigned)(items * a.pool.nkv));
         if (form == 0) hipLaunchKernelGGL((k_pages_attn<FMT, D, 1>), grid, dim3(256), 0, st, a);
-        else hipLaunchKernelGGL((k_pages_attn<FMT, D, 2>), grid, dim3(256), 0, st, a);
+        else if (form == 1) hipLaunchKernelGGL((k_pages_attn<FMT, D, 2>), grid, dim3(256), 0, st, a);
+        else if constexpr (FMT == FL_KV_F16) {
+            // two steps of K and V, or the waves' results
+            constexpr size_t lds = std::max(2 * 8 * 32 * D * 2, 8 * 32 * (D + 4) * 4);
+            if (form == 2) hipLaunchKernelGGL((k_pages_wide<D, 2>), grid, dim3(512), lds, st, a);
+            else hipLaunchKernelGGL((k_pages_wide<D, 4>), grid, dim3(512), lds, st, a);
+        }
         return (int)hipGetLastError();
     }
 };
@@ -221,10 +234,11 @@ struct LaunchAttn {
 struct LaunchWrite {
     hipStream_t st;
     const PageWriteArgs &a;
+    const PageSlots &slots;
     template <int FMT, int D>
     int operator()() const {
         const long long total = (long long)a.layers * a.n * a.pool.nkv * (D / 32) * 2;
-        hipLaunchKernelGGL((k_pages_write<FMT, D>), dim3((unsigned)((total + 255) / 256)), dim3(256), 0, st, a);
+        hipLaunchKernelGGL((k_pages_write<FMT, D>), dim3((unsigned)((total + 255) / 256)), dim3(256), 0, st, a, slots);
         return (int)hipGetLastError();
     }
 };
@@ -240,6 +254,8 @@ struct LaunchRead {
     }
 };
 
+int forms_of(const fl_pages *p) { return p->cfg.kv_format == FL_KV_F16 ? 4 : 2; }
+
 // The plan of these queries, on the device.
 int make_plan(fl_pages *p, const int32_t *seqs, const int32_t *seen, int n, int heads) {
     const int group = heads / p->cfg.num_kv_heads;
@@ -248,7 +264,7 @@ int make_plan(fl_pages *p, const int32_t *seqs, const int32_t *seen, int n, int 
         return 0;
     p->plan_version = 0;
     PGTRY(on_table(p, [&](PageTable &t) {
-        const int rc = page_plan(t, seqs, seen, n, group, p->cfg.num_kv_heads, p->plan);
+        const int rc = page_plan(t, seqs, seen, n, group, p->cfg.num_kv_heads, forms_of(p), p->plan);
         if (rc) return rc;
         p->plan_seqs.assign(seqs, seqs + n);
         p->plan_seen.assign(seen, seen + n);
@@ -261,7 +277,7 @@ int make_plan(fl_pages *p, const int32_t *seqs, const int32_t *seen, int n, int 
         bytes = (bytes + b + 63) / 64 * 64;
         return at;
     };
-    for (int f = 0; f < kPageTiles; f++) p->plan_items[f] = place(l.items[f].size() * sizeof(PageItem));
+    for (int f = 0; f < kPageForms; f++) p->plan_items[f] = place(l.items[f].size() * sizeof(PageItem));
     p->plan_order = place(l.order.size() * sizeof(PageQuery));
     p->plan_pages = place(l.page_ids.size() * sizeof(int));
     p->plan_units = place(l.units.size() * sizeof(int));
@@ -273,7 +289,7 @@ int make_plan(fl_pages *p, const int32_t *seqs, const int32_t *seen, int n, int 
     auto put = [&](size_t at, const auto &v) {
         if (!v.empty()) memcpy(h + at, v.data(), v.size() * sizeof v[0]);
     };
-    for (int f = 0; f < kPageTiles; f++) put(p->plan_items[f], l.items[f]);
+    for (int f = 0; f < kPageForms; f++) put(p->plan_items[f], l.items[f]);
     put(p->plan_order, l.order);
     put(p->plan_pages, l.page_ids);
     put(p->plan_units, l.units);
@@ -322,7 +338,7 @@ int fl_pages_create(fl_ctx *ctx, const fl_pages_config *cfg, void *k, void *v, v
         p->stream = (hipStream_t)fl_ctx_stream(ctx);
     }
     int rc = on_table(p, [&](PageTable &t) { return t.init(*cfg); });
-    if (!rc && ctx) {
+    if (!rc && ctx && cfg->num_pages > kInlineCopies) {
         OnDevice on(p);
         // (a call's copies go to as many pages at most, so this never fails later)
         rc = ensure(p, p->d_copies, (size_t)cfg->num_pages * sizeof(PageCopy));
@@ -388,9 +404,9 @@ int fl_pages_extend(fl_pages *p, const int32_t *seqs, const int32_t *counts, int
     long long tokens = 0;
     for (int i = 0; i < n && counts; i++) tokens += std::min(std::max(counts[i], 0), p->cfg.max_seq_len);
     tokens = std::min(tokens, (long long)p->cfg.num_pages * p->cfg.page_size);
-    PGTRY(ensure(p, p->d_slots, (size_t)tokens * sizeof(int)));
+    if (tokens > kInlineSlots) PGTRY(ensure(p, p->d_slots, (size_t)tokens * sizeof(int)));
     PGTRY(on_table(p, [&](PageTable &t) { return t.extend(seqs, counts, n); }));
-    if (!p->t.slots.empty()) PGTRY(upload(p, p->d_slots, p->t.slots.data(), p->t.slots.size() * sizeof(int)));
+    if (p->t.slots.size() > kInlineSlots) PGTRY(upload(p, p->d_slots, p->t.slots.data(), p->t.slots.size() * sizeof(int)));
     return run_copies(p);
 }
 
@@ -407,14 +423,17 @@ int fl_pages_write(fl_pages *p, int layer, int layers, const float *k, const flo
     OnDevice on(p);
     PageWriteArgs a{};
     a.pool = p->pool;
-    a.slots = (const int *)p->d_slots.p;
+    PageSlots slots;
+    slots.list = nullptr;
+    if (p->t.slots.size() > kInlineSlots) slots.list = (const int *)p->d_slots.p;
+    else memcpy(slots.some, p->t.slots.data(), p->t.slots.size() * sizeof(int));
     a.k = k;
     a.v = v;
     a.stride = (long long)row_stride;
     a.layer0 = layer;
     a.layers = layers;
     a.n = (int)p->t.slots.size();
-    PGCHK(p, (hipError_t)with_form(p->cfg.kv_format, p->cfg.head_dim, LaunchWrite{p->stream, a}));
+    PGCHK(p, (hipError_t)with_form(p->cfg.kv_format, p->cfg.head_dim, LaunchWrite{p->stream, a, slots}));
     return 0;
 }
 
@@ -460,7 +479,7 @@ int fl_pages_attention(fl_pages *p, int layer, const float *q, size_t q_stride, 
     PGTRY(check_layers(p, layer, 1));
     const int D = p->cfg.head_dim, nkv = p->cfg.num_kv_heads;
     if (num_heads < 1 || num_heads % nkv) return fail(p, FL_E_INVALID, "%d heads over %d kv heads", num_heads, nkv);
-    if (num_heads / nkv > 16 * kPageTiles) return fail(p, FL_E_UNSUPPORTED, "%d query heads per kv head", num_heads / nkv);
+    if (num_heads / nkv > kPageRows[1]) return fail(p, FL_E_UNSUPPORTED, "%d query heads per kv head", num_heads / nkv);
     if (n < 0) return fail(p, FL_E_INVALID, "%d queries", n);
     if (n == 0) return 0;
     if (!q || !out || !seqs || !seen) return fail(p, FL_E_INVALID, "null argument");
@@ -483,7 +502,7 @@ int fl_pages_attention(fl_pages *p, int layer, const float *q, size_t q_stride, 
     a.part = (float *)p->ws.p;
     a.ml = a.part + (size_t)l.num_units * num_heads * D;
     a.out = out;
-    for (int f = kPageTiles - 1; f >= 0; f--) {
+    for (int f = kPageForms - 1; f >= 0; f--) {
         if (l.items[f].empty()) continue;
         a.items = (const PageItem *)(d + p->plan_items[f]);
         PGCHK(p, (hipError_t)with_form(p->cfg.kv_format, D, LaunchAttn{p->stream, a, (int)l.items[f].size(), f}));
@@ -499,6 +518,8 @@ int fl_pages_attention(fl_pages *p, int layer, const float *q, size_t q_stride, 
 }
 
 int fl_pages_len(const fl_pages *p, int seq) { return p && seq >= 0 && seq < p->t.seqs ? p->t.len[seq] : -1; }
+
+int fl_pages_pending(const fl_pages *p) { return p && p->t.slots_valid ? (int)p->t.slots.size() : -1; }
 
 int fl_pages_free_count(const fl_pages *p) { return p ? p->t.free_pages : -1; }
 
@@ -523,14 +544,14 @@ int fl_pages_copies(const fl_pages *p, int32_t *copies, int cap) {
 int fl_pages_plan(fl_pages *p, const int32_t *seqs, const int32_t *seen, int n, int num_heads, int32_t *items, int cap) {
     if (!p) return fail(p, FL_E_INVALID, "null pages");
     const int nkv = p->cfg.num_kv_heads;
-    if (num_heads < 1 || num_heads % nkv || num_heads / nkv > 16 * kPageTiles)
+    if (num_heads < 1 || num_heads % nkv || num_heads / nkv > kPageRows[1])
         return fail(p, FL_E_INVALID, "%d heads over %d kv heads", num_heads, nkv);
     int made = 0;
     PGTRY(on_table(p, [&](PageTable &t) {
         PagePlan l;
-        const int rc = page_plan(t, seqs, seen, n, num_heads / nkv, nkv, l);
+        const int rc = page_plan(t, seqs, seen, n, num_heads / nkv, nkv, forms_of(p), l);
         if (rc) return rc;
-        for (int f = 0; f < kPageTiles; f++)
+        for (int f = 0; f < kPageForms; f++)
             for (const PageItem &it : l.items[f])
                 for (int i = 0; i < it.nq; i++, made++) {
                     if (!items || made >= cap) continue;

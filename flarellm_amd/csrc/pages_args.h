@@ -37,9 +37,20 @@ struct PageJoinArgs {
     int heads;
 };
 
+// Short lists go with the launch (a copy to the device costs the host 5 us and the
+// stream 3); longer ones are in device memory.
+constexpr int kInlineSlots = 256, kInlineCopies = 96;
+struct PageSlots {
+    const int *list;       // page * P + slot of each token; nullptr: `some`
+    int some[kInlineSlots];
+};
+struct PageCopies {
+    const PageCopy *list;  // nullptr: `some`
+    PageCopy some[kInlineCopies];
+};
+
 struct PageWriteArgs {
     PagePool pool;
-    const int *slots;      // page * P + slot of each token
     const float *k, *v;    // token i, kv head h at (layer * n + i) * stride + h * D
     long long stride;
     int layer0, layers, n;

@@ -245,7 +245,8 @@ int PageTable::compact() {
 // them.  A run's queries, longest first, are cut into tiles of up to 32 rows (query
 // x head of a kv head) and its tokens into parts, until the chip is full.
 // ---------------------------------------------------------------------------
-int page_plan(PageTable &t, const int32_t *s, const int32_t *seen, int n, int group, int kv_heads, PagePlan &p) {
+int page_plan(PageTable &t, const int32_t *s, const int32_t *seen, int n, int group, int kv_heads, int forms,
+              PagePlan &p) {
     auto fail = [&](int code, const std::string &m) {
         t.error = m;
         return code;
@@ -299,7 +300,7 @@ int page_plan(PageTable &t, const int32_t *s, const int32_t *seen, int n, int gr
     };
     std::vector<Run> todo{{0, (int)seqs.size(), 0, 0}};
     std::vector<Tile> tiles;
-    const int most = std::max(1, 16 * kPageTiles / group);  // queries of the largest tile
+    const int most = std::max(1, kPageRows[forms - 1] / group);  // queries of the largest tile
     while (!todo.empty()) {
         Run r = todo.back();
         todo.pop_back();
@@ -336,20 +337,24 @@ int page_plan(PageTable &t, const int32_t *s, const int32_t *seen, int n, int gr
         for (int i = r.p0; i < e; i++) p.page_ids.push_back(seqs[r.lo].pages[i]);
         for (int i = 0; i < total; i += most) {
             const int nq = std::min(most, total - i);
-            tiles.push_back({first + i, nq, from, std::min(p.order[first + i].seen, end), page0,
-                             std::min(kPageTiles, ceil_div(nq * group, 16)) - 1});
+            int form = 0;
+            while (kPageRows[form] < nq * group) form++;
+            tiles.push_back({first + i, nq, from, std::min(p.order[first + i].seen, end), page0, form});
         }
     }
 
-    // Parts: about kPageFill workgroups, none of less than kPageLeast blocks
+    // Parts: about so many workgroups, none of less than so many blocks
     constexpr int kPageFill = 768, kPageLeast = 8;
-    long long blocks = 0;
-    for (const Tile &x : tiles) blocks += ceil_div(x.slot1 - x.slot0, kPageBlock);
-    const int part = (int)std::max<long long>(kPageLeast, (blocks * kv_heads + kPageFill - 1) / kPageFill);
+    constexpr int kWideFill = 256, kWideLeast = 16;
+    long long blocks[2] = {0, 0};
+    for (const Tile &x : tiles) blocks[x.form > 1] += ceil_div(x.slot1 - x.slot0, kPageBlock);
+    const int parts[2] = {(int)std::max<long long>(kPageLeast, (blocks[0] * kv_heads + kPageFill - 1) / kPageFill),
+                          (int)std::max<long long>(kWideLeast, (blocks[1] * kv_heads + kWideFill - 1) / kWideFill)};
     std::vector<int> count(n, 0);
     std::vector<std::pair<int, int>> at;  // form and index of every item
     for (const Tile &x : tiles) {
-        const int nb = ceil_div(x.slot1 - x.slot0, kPageBlock), cuts = ceil_div(nb, part), each = ceil_div(nb, cuts);
+        const int nb = ceil_div(x.slot1 - x.slot0, kPageBlock), cuts = ceil_div(nb, parts[x.form > 1]);
+        const int each = ceil_div(nb, cuts);
         for (int b = 0; b < nb; b += each) {
             PageItem it{};
             it.q0 = x.q0;

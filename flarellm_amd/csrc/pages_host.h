@@ -77,10 +77,11 @@ struct PageJoin {
     int query, first, count, pad;
 };
 
-constexpr int kPageTiles = 2;  // item forms: up to 16 and up to 32 rows (query x head of a kv head)
+// Item forms, by rows (query x head of a kv head): one and two tiles of 16, 2 and 4 of 32.
+constexpr int kPageForms = 4, kPageRows[kPageForms] = {16, 32, 64, 128};
 
 struct PagePlan {
-    std::vector<PageItem> items[kPageTiles];
+    std::vector<PageItem> items[kPageForms];
     std::vector<PageQuery> order;
     std::vector<int> page_ids, units;
     std::vector<PageJoin> joins;
@@ -88,7 +89,8 @@ struct PagePlan {
 };
 
 // seen[i] tokens of sequence s[i] for query i (checked against the table).
-// group: query heads per kv head.  0, or a code and table.error.
-int page_plan(PageTable &t, const int32_t *s, const int32_t *seen, int n, int group, int kv_heads, PagePlan &p);
+// group: query heads per kv head; forms: how many of the item forms there are.  0, or a
+// code and table.error.
+int page_plan(PageTable &t, const int32_t *s, const int32_t *seen, int n, int group, int kv_heads, int forms, PagePlan &p);
 
 }  // namespace fl

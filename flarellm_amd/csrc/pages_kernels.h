@@ -2,17 +2,23 @@
 // their sequences, and the stores, reads and copies of pages.
 #pragma once
 
+#include "bgemm_pack.h"
 #include "pages_args.h"
 
 namespace fl {
 
 typedef _Float16 ph8_t __attribute__((ext_vector_type(8)));
 typedef float pf4_t __attribute__((ext_vector_type(4)));
+typedef float pf16_t __attribute__((ext_vector_type(16)));
 typedef uint32_t pu4_t __attribute__((ext_vector_type(4)));
 typedef uint32_t pu2_t __attribute__((ext_vector_type(2)));
 
 __device__ __forceinline__ pf4_t pg_mfma_h(pu4_t a, pu4_t b, pf4_t c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(ph8_t, a), __builtin_bit_cast(ph8_t, b), c, 0, 0, 0);
+}
+
+__device__ __forceinline__ pf16_t pg_mfma_w(pu4_t a, pu4_t b, pf16_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(ph8_t, a), __builtin_bit_cast(ph8_t, b), c, 0, 0, 0);
 }
 
 // 8 floats as two binary16 parts (round toward zero, then the rest)
@@ -24,6 +30,17 @@ __device__ __forceinline__ void pg_split(const float *x, pu4_t &hi, pu4_t &lo) {
         hi[i] = __builtin_bit_cast(uint32_t, h);
         lo[i] = __builtin_bit_cast(uint32_t, l);
     }
+}
+
+// A power of two that brings a query's largest value x to 2^13, so that the low parts
+// of the others stay normal (zero, denormal and non-finite rows stay), and the score
+// scale c for it.
+__device__ __forceinline__ void pg_q_scale(float x, float &mul, float &c) {
+    const int e = (int)((__float_as_uint(x) >> 23) & 0xFF);
+    if (e <= 13 || e == 255) return;
+    const int s = min(max(140 - e, -100), 100);
+    mul = __uint_as_float((uint32_t)(127 + s) << 23);
+    c *= __uint_as_float((uint32_t)(127 - s) << 23);
 }
 
 // 8 signed bytes as 8 binary16 values, exactly: byte b ^ 0x80 under the exponent of
@@ -65,6 +82,20 @@ __device__ __forceinline__ float pg_v(const PagePool &p, size_t head, int slot, 
     if constexpr (FMT == FL_KV_F16) return h2f(((const uint16_t *)p.v)[e]);
     return (float)((const int8_t *)p.v)[e] * h2f(p.vs[(head * p.P + slot) * (D / 32) + (d >> 5)]);
 }
+
+// Scale of a block of 32 channels, and the factor that its codes are rounded from:
+// amax / 127 and 127 / amax from one division (quantize_input_q8_0_into, model.rs:
+// 5557-5570, has two: a scale may differ from its in the last place, a code by one
+// where the value is next to a half).
+__device__ __forceinline__ void pg_q8_scale(float amax, float &scale, float &factor) {
+    scale = amax * (1.0f / 127.0f);
+    asm("" : "+v"(scale));  // rounded to f32 before binary16 (not v_fma_mixlo_f16's one rounding)
+    factor = amax > 0.0f ? 1.0f / amax * 127.0f : 0.0f;
+}
+
+// p is kept times 2^15 where its parts are binary16, so that they hold 22 bits down to 2^-18
+template <int FMT>
+constexpr float kPageShift = FMT == FL_KV_F32 ? 0.0f : 15.0f;
 
 // The operands of a 32-slot block of one (page, kv head), in registers.  Scores are
 // formed transposed, S^T = K Q^T, with 16 x 16 products: a query row is a lane (mod
@@ -263,6 +294,103 @@ struct PgBlock<FL_KV_F32, D> {
     }
 };
 
+// An item's rows key by key, where some value was not finite: 2^kShift times the
+// sum and O, in base 2 relative to the largest score, as the tiles have them (all rows
+// of the item; this is rare).  lds: 260 floats.
+template <int FMT, int D>
+__device__ __forceinline__ void pg_rows_again(const PageAttnArgs &a, const PageItem &it, int kvh, float *lds) {
+    const int nkv = a.pool.nkv, G = a.group, nh = nkv * G, P = a.pool.P, rows = it.nq * G;
+    const size_t layer_pages = (size_t)a.layer * a.pool.pages;
+    const int tid = threadIdx.x;
+    float *sc = lds, *red = lds + 256;
+    auto head_of = [&](int t) { return (layer_pages + a.page_ids[it.page0 + t / P - it.slot0 / P]) * nkv + kvh; };
+    for (int row = 0; row < rows; row++) {
+        const int qi = row / G, hd = kvh * G + row % G;
+        const PageQuery pq = a.order[it.q0 + qi];
+        const float *qp = a.q + pq.query * a.q_stride + (size_t)hd * D;
+        const int end = min(pq.seen, it.slot1);
+        float mx = -INFINITY, sum = 0.0f, acc = 0.0f;
+        for (int t0 = it.slot0; t0 < end; t0 += 256) {
+            const int t = t0 + tid;
+            float x = -INFINITY;
+            if (tid < 256 && t < end) {
+                x = 0.0f;
+                for (int d = 0; d < D; d++) x = __builtin_fmaf(qp[d], pg_k<FMT, D>(a.pool, head_of(t), t % P, d), x);
+                x *= a.scale;
+            }
+            __syncthreads();
+            if (tid < 256) sc[tid] = x;
+            for (int i = 1; i < 64; i <<= 1) x = fmaxf(x, __shfl_xor(x, i, 64));
+            if (tid < 256 && (tid & 63) == 0) red[tid >> 6] = x;
+            __syncthreads();
+            const float mn = fmaxf(mx, fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])));
+            const float al = mx == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mx - mn);
+            sum *= al;
+            acc *= al;
+            mx = mn;
+            for (int i = 0; i < 256 && t0 + i < end; i++) {
+                const float y = sc[i], p = y == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(y - mx + kPageShift<FMT>);
+                sum += p;
+                if (tid < D) acc = __builtin_fmaf(p, pg_v<FMT, D>(a.pool, head_of(t0 + i), (t0 + i) % P, tid), acc);
+            }
+        }
+        __syncthreads();
+        if (tid >= D) continue;
+        if (it.unit < 0) {
+            a.out[((size_t)pq.query * nh + hd) * D + tid] = acc / sum;
+        } else {
+            const size_t u = (size_t)(it.unit + qi) * nh + hd;
+            a.part[u * D + tid] = acc;
+            if (tid == 0) {
+                a.ml[u * 2] = mx;
+                a.ml[u * 2 + 1] = sum;
+            }
+        }
+    }
+}
+
+// A row of an item's result: channels ch .. ch + N - 1 from the KL partial results at
+// lds[i * step], each [D] O, max, sum.  Sets *bad where a value is not finite.
+template <int D, int N, int KL>
+__device__ __forceinline__ void pg_join_row(const PageAttnArgs &a, const PageItem &it, int kvh, int row, int ch,
+                                            const float *lds, int step, int *bad) {
+    float mx = -INFINITY, sum = 0.0f, wt[KL];
+#pragma unroll
+    for (int i = 0; i < KL; i++) mx = fmaxf(mx, lds[i * step + D]);
+#pragma unroll
+    for (int i = 0; i < KL; i++) {
+        const float mi = lds[i * step + D];
+        wt[i] = mi == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mi - mx);
+        sum = __builtin_fmaf(lds[i * step + D + 1], wt[i], sum);
+    }
+    float odd = sum * 0.0f;
+    const int G = a.group, nh = a.pool.nkv * G, qi = row / G, hd = kvh * G + row % G;
+    const size_t u = (size_t)(it.unit < 0 ? a.order[it.q0 + qi].query : it.unit + qi) * nh + hd;
+    float *op = (it.unit < 0 ? a.out : a.part) + u * D + ch;
+    const float il = it.unit < 0 ? 1.0f / sum : 1.0f;
+#pragma unroll
+    for (int j = 0; j < N; j += 4) {
+        pf4_t y = {0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < KL; i++) {
+            const pf4_t x = *(const pf4_t *)(lds + i * step + ch + j);
+#pragma unroll
+            for (int k = 0; k < 4; k++) y[k] = __builtin_fmaf(x[k], wt[i], y[k]);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            y[k] *= il;
+            odd = __builtin_fmaf(y[k], 0.0f, odd);
+        }
+        *(pf4_t *)(op + j) = y;
+    }
+    if (it.unit >= 0 && ch == 0) {
+        a.ml[u * 2] = mx;
+        a.ml[u * 2 + 1] = sum;
+    }
+    if (odd != 0.0f) *bad = 1;  // 0 * Inf and 0 * NaN are NaN
+}
+
 // One item (PageItem) and kv head per workgroup of 4 waves; wave w takes the item's
 // 32-slot blocks w, w + 4, ..  Each keeps (max, sum, O) of its blocks for NT x 16
 // rows (query x head), joined through LDS at the end.  K of a wave's next block is
@@ -276,7 +404,6 @@ template <int FMT, int D, int NT>
 __global__ __launch_bounds__(256) void k_pages_attn(PageAttnArgs a) {
     using Block = PgBlock<FMT, D>;
     constexpr int QP = Block::QP, DT = D / 16;
-    constexpr float kShift = FMT == FL_KV_F32 ? 0.0f : 15.0f;  // p is kept times 2^15: its parts hold 22 bits
     // [4 waves][16 rows][D + 4]: O, max, sum (of one 16-row tile at a time)
     constexpr int LROW = D + 4;
     __shared__ __align__(16) float lds[4 * 16 * LROW];
@@ -318,19 +445,12 @@ __global__ __launch_bounds__(256) void k_pages_attn(PageAttnArgs a) {
         c[n] = a.scale;
         float mul = 1.0f;
         if constexpr (FMT != FL_KV_F32) {
-            // the row's largest value is brought to 2^13, so that the low parts stay normal
             float x = 0.0f;
 #pragma unroll
             for (int k = 0; k < D / 32; k++)
 #pragma unroll
                 for (int j = 0; j < 8; j++) x = fmaxf(x, fabsf(qp[32 * k + 8 * g + j]));
-            x = pg_max16(x);
-            const int e = (int)((__float_as_uint(x) >> 23) & 0xFF);
-            if (e > 13 && e < 255) {
-                const int s = min(max(140 - e, -100), 100);
-                mul = __uint_as_float((uint32_t)(127 + s) << 23);
-                c[n] *= __uint_as_float((uint32_t)(127 - s) << 23);
-            }
+            pg_q_scale(pg_max16(x), mul, c[n]);
         }
         Block::make_q(qp, mul, g, q[n]);
     }
@@ -378,7 +498,7 @@ __global__ __launch_bounds__(256) void k_pages_attn(PageAttnArgs a) {
                     for (int i = 0; i < 4; i++) o[n][d][i] *= al;
             }
             // a row that has seen no token yet keeps p = 0
-            const float off = m_run[n] == -INFINITY ? -INFINITY : kShift - m_run[n];
+            const float off = m_run[n] == -INFINITY ? -INFINITY : kPageShift<FMT> - m_run[n];
             float p[8];
 #pragma unroll
             for (int j = 0; j < 8; j++) {
@@ -406,132 +526,228 @@ __global__ __launch_bounds__(256) void k_pages_attn(PageAttnArgs a) {
             w[D + 1] = l;
         }
         __syncthreads();
-        const int r = threadIdx.x >> 4, ch = (threadIdx.x & 15) * (D / 16), row = 16 * n + r;
-        float mx = -INFINITY, sum = 0.0f, wt[4];
+        const int r = threadIdx.x >> 4, row = 16 * n + r;
+        if (row < rows)
+            pg_join_row<D, D / 16, 4>(a, it, kvh, row, (threadIdx.x & 15) * (D / 16), lds + r * LROW, 16 * LROW, &bad_rows);
+    }
+    __syncthreads();
+    if (bad_rows) pg_rows_again<FMT, D>(a, it, kvh, lds);
+}
+
+// Items of 33 to 32 R rows (R = 2, 4): 8 waves, R row groups of 32 x 8 / R key lanes.
+// A step is 128 tokens, K and V of its four 32-slot blocks copied memory -> LDS one step
+// ahead (wave w copies K or V of one block); a key lane takes R / 2 of them.  Products are
+// 32 x 32 x 16: a query row is a lane (mod 32), the K rows enter with index bits 2 and 3
+// swapped so that scores i = 8 mm + j of a lane are slots 16 mm + 8 (lane / 32) + j, the
+// operand of O^T = V^T P^T.  Bound by the matrix issue: 64 products of 32 cycles per block
+// and row group, two waves a SIMD, whose softmax runs beside the other's products.
+template <int D, int R>
+__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) void k_pages_wide(PageAttnArgs a) {
+    constexpr int FMT = FL_KV_F16, KL = 8 / R, NB = 4 / KL;
+    constexpr int KS = D / 16, DT = D / 32, CH = D / 8, BLK = 32 * D * 2;  // BLK: bytes of a block's K (or V)
+    constexpr int LROW = D + 4;
+    extern __shared__ __align__(16) char smem[];  // 2 x (4 K blocks, 4 V blocks); at the end [8 waves][32][LROW]
+    __shared__ int bad_rows;
+    const int lane = threadIdx.x & 63, l31 = lane & 31, h = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), rg = wave % R, kl = wave / R;
+    const int nkv = a.pool.nkv, kvh = blockIdx.x % nkv, G = a.group;
+    const PageItem it = a.items[blockIdx.x / nkv];
+    const int rows = it.nq * G, P = a.pool.P;
+    const int nb = (it.slot1 - it.slot0 + 31) >> 5, nit = (nb + 3) >> 2;
+    const size_t layer_pages = (size_t)a.layer * a.pool.pages;
+    const bool live = 32 * rg < rows;  // wave-uniform
+    if (threadIdx.x == 0) bad_rows = 0;
+
+    // chunk p (16 B) of a K block in LDS holds chunk c ^ g(row) of its row, g from row bits
+    // 0, 1, 3 (the rows that 8 lanes read together differ in those); of a V block, chunk
+    // c ^ (channel >> 1 & 3) of its channel
+    auto copy = [&](int step, int buf) {
+        const int w = wave & 3, b = min(4 * step + w, nb - 1), tok = it.slot0 + 32 * b;
+        const int page = __builtin_amdgcn_readfirstlane(a.page_ids[it.page0 + tok / P - it.slot0 / P]);
+        const size_t at = (((layer_pages + page) * nkv + kvh) * P + tok % P) * D * 2;
+        const char *src = (const char *)(wave < 4 ? a.pool.k : a.pool.v) + at;
+        char *dst = smem + (size_t)(8 * buf + wave) * BLK;
 #pragma unroll
-        for (int i = 0; i < 4; i++) mx = fmaxf(mx, lds[(16 * i + r) * LROW + D]);
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const float mi = lds[(16 * i + r) * LROW + D];
-            wt[i] = mi == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mi - mx);
-            sum = __builtin_fmaf(lds[(16 * i + r) * LROW + D + 1], wt[i], sum);
+        for (int u = 0; u < BLK / 1024; u++) {
+            const int p = 64 * u + lane, r = p / CH, g = (r & 3) | ((r >> 1) & 4);
+            const int off = wave < 4 ? r * CH + ((p % CH) ^ g) : (p & ~3) | ((p & 3) ^ ((p >> 3) & 3));
+            copy_to_lds(src + off * 16, dst + u * 1024);
         }
-        float y[D / 16], odd = sum * 0.0f;
+    };
+    copy(0, 0);
+
+    const int r0 = min(32 * rg + l31, rows - 1);
+    const PageQuery pq = a.order[it.q0 + r0 / G];
+    const float *qp = a.q + pq.query * a.q_stride + (size_t)(kvh * G + r0 % G) * D + 8 * h;
+    float c = a.scale, mul = 1.0f, x0 = 0.0f;
 #pragma unroll
-        for (int j = 0; j < D / 16; j++) y[j] = 0.0f;
+    for (int k = 0; k < KS; k++)
 #pragma unroll
-        for (int i = 0; i < 4; i++)
+        for (int j = 0; j < 8; j++) x0 = fmaxf(x0, fabsf(qp[16 * k + j]));
+    pg_q_scale(fmaxf(x0, __shfl_xor(x0, 32, 64)), mul, c);
+    pu4_t q[KS][2];
 #pragma unroll
-            for (int j = 0; j < D / 16; j++) y[j] = __builtin_fmaf(lds[(16 * i + r) * LROW + ch + j], wt[i], y[j]);
-        const float il = it.unit < 0 ? 1.0f / sum : 1.0f;
+    for (int k = 0; k < KS; k++) {
+        float x[8];
 #pragma unroll
-        for (int j = 0; j < D / 16; j++) {
-            y[j] *= il;
-            odd = __builtin_fmaf(y[j], 0.0f, odd);
+        for (int j = 0; j < 8; j++) x[j] = qp[16 * k + j] * mul;
+        pg_split(x, q[k][0], q[k][1]);
+    }
+    const pf16_t zero = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+    pf16_t o[DT];
+#pragma unroll
+    for (int d = 0; d < DT; d++) o[d] = zero;
+    float m_run = -INFINITY, l_run = 0.0f;
+    const int krow = (l31 & 0x13) | ((l31 & 4) << 1) | ((l31 & 8) >> 1);
+    const int kg = (krow & 3) | ((krow >> 1) & 4);
+
+    for (int step = 0; step < nit; step++) {
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();  // this step has landed, and nobody reads the other buffer
+        asm volatile("" ::: "memory");
+        const int buf = step & 1;
+        if (step + 1 < nit) {
+            copy(step + 1, buf ^ 1);
+        } else if (const int over = (it.slot1 - it.slot0) & 31; over) {
+            // slots behind the item's last token: whatever is there must not meet a zero
+            char *vb = smem + (size_t)(8 * buf + 4 + ((nb - 1) & 3)) * BLK;
+            for (int i = threadIdx.x; i < 32 * D; i += 512) {
+                const int d = i >> 5, s = i & 31;
+                if (s >= over) *(uint16_t *)(vb + d * 64 + (((s >> 3) ^ ((d >> 1) & 3)) * 16) + (s & 7) * 2) = 0;
+            }
+            __syncthreads();
         }
-        if (row < rows) {
-            const int qi = row / G, hd = kvh * G + row % G;
-            float *op;
-            if (it.unit < 0) {
-                op = a.out + ((size_t)a.order[it.q0 + qi].query * nh + hd) * D;
-            } else {
-                op = a.part + ((size_t)(it.unit + qi) * nh + hd) * D;
-                if (ch == 0) {
-                    float *ml = a.ml + ((size_t)(it.unit + qi) * nh + hd) * 2;
-                    ml[0] = mx;
-                    ml[1] = sum;
-                }
+        if (!live) continue;
+#pragma unroll 1
+        for (int i = 0; i < NB; i++) {
+            const int bi = NB * kl + i, tok = it.slot0 + 32 * (4 * step + bi);
+            if (tok >= it.slot1) break;
+            const char *kt = smem + (size_t)(8 * buf + bi) * BLK + krow * D * 2, *vt = smem + (size_t)(8 * buf + 4 + bi) * BLK;
+            pf16_t s = zero, lo = zero;
+#pragma unroll
+            for (int k = 0; k < KS; k++) {
+                const pu4_t kf = *(const pu4_t *)(kt + (((2 * k + h) ^ kg) * 16));
+                lo = pg_mfma_w(kf, q[k][1], lo);
+                s = pg_mfma_w(kf, q[k][0], s);
             }
 #pragma unroll
-            for (int j = 0; j < D / 16; j += 4) *(pf4_t *)(op + ch + j) = pf4_t{y[j], y[j + 1], y[j + 2], y[j + 3]};
-            if (odd != 0.0f) bad_rows = 1;  // 0 * Inf and 0 * NaN are NaN
+            for (int j = 0; j < 16; j++) s[j] += lo[j];
+            if (tok + 32 > it.smin) {  // some query does not see every token
+                const int end = min(pq.seen, it.slot1) - tok;
+#pragma unroll
+                for (int j = 0; j < 16; j++)
+                    if (16 * (j >> 3) + 8 * h + (j & 7) >= end) s[j] = -INFINITY;
+            }
+            float m = s[0];
+#pragma unroll
+            for (int j = 1; j < 16; j++) m = fmaxf(m, s[j]);
+            m = fmaxf(m, __shfl_xor(m, 32, 64)) * c;
+            if (__any(m > m_run)) {
+                const float mn = fmaxf(m_run, m);
+                const float al = m_run == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m_run - mn);
+                m_run = mn;
+                l_run *= al;
+#pragma unroll
+                for (int d = 0; d < DT; d++)
+#pragma unroll
+                    for (int j = 0; j < 16; j++) o[d][j] *= al;
+            }
+            // a row that has seen no token yet keeps p = 0 (a score of -Inf makes the exponent -Inf, too)
+            const float off = m_run == -INFINITY ? -INFINITY : kPageShift<FMT> - m_run;
+            float p[16];
+#pragma unroll
+            for (int j = 0; j < 16; j++) {
+                p[j] = __builtin_amdgcn_exp2f(s[j] == -INFINITY ? -INFINITY : __builtin_fmaf(s[j], c, off));
+                l_run += p[j];
+            }
+            pu4_t pf[2][2];
+            pg_split(p, pf[0][0], pf[0][1]);
+            pg_split(p + 8, pf[1][0], pf[1][1]);
+#pragma unroll
+            for (int d = 0; d < DT; d++) {
+                const int dd = 32 * d + l31;
+#pragma unroll
+                for (int mm = 0; mm < 2; mm++) {
+                    const pu4_t vf = *(const pu4_t *)(vt + dd * 64 + (((2 * mm + h) ^ ((dd >> 1) & 3)) * 16));
+                    o[d] = pg_mfma_w(vf, pf[mm][1], o[d]);
+                    o[d] = pg_mfma_w(vf, pf[mm][0], o[d]);
+                }
+            }
         }
     }
     __syncthreads();
-    if (!bad_rows) return;
-
-    // Rows key by key, in the same terms: max of scores in base 2, sum and O times
-    // 2^kShift (all rows of the item; this is rare).
-    float *sc = lds, *red = lds + 256;
-    for (int row = 0; row < rows; row++) {
-        const int qi = row / G, hd = kvh * G + row % G;
-        const PageQuery pq = a.order[it.q0 + qi];
-        const float *qp = a.q + pq.query * a.q_stride + (size_t)hd * D;
-        const int end = min(pq.seen, it.slot1);
-        float mx = -INFINITY, sum = 0.0f, acc = 0.0f;
-        for (int t0 = it.slot0; t0 < end; t0 += 256) {
-            const int t = t0 + threadIdx.x;
-            float x = -INFINITY;
-            if (t < end) {
-                const size_t h = (layer_pages + a.page_ids[it.page0 + t / P - it.slot0 / P]) * nkv + kvh;
-                x = 0.0f;
-                for (int d = 0; d < D; d++) x = __builtin_fmaf(qp[d], pg_k<FMT, D>(a.pool, h, t % P, d), x);
-                x *= a.scale;
-            }
-            __syncthreads();
-            sc[threadIdx.x] = x;
-            for (int i = 1; i < 64; i <<= 1) x = fmaxf(x, __shfl_xor(x, i, 64));
-            if (lane == 0) red[wave] = x;
-            __syncthreads();
-            const float mn = fmaxf(mx, fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])));
-            const float al = mx == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mx - mn);
-            sum *= al;
-            acc *= al;
-            mx = mn;
-            for (int i = 0; i < 256 && t0 + i < end; i++) {
-                const float y = sc[i], p = y == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(y - mx + kShift);
-                sum += p;
-                if (threadIdx.x < D) {
-                    const int t2 = t0 + i;
-                    const size_t h = (layer_pages + a.page_ids[it.page0 + t2 / P - it.slot0 / P]) * nkv + kvh;
-                    acc = __builtin_fmaf(p, pg_v<FMT, D>(a.pool, h, t2 % P, threadIdx.x), acc);
-                }
-            }
-        }
-        __syncthreads();
-        if (threadIdx.x < D) {
-            if (it.unit < 0) {
-                a.out[((size_t)pq.query * nh + hd) * D + threadIdx.x] = acc / sum;
-            } else {
-                const size_t u = (size_t)(it.unit + qi) * nh + hd;
-                a.part[u * D + threadIdx.x] = acc;
-                if (threadIdx.x == 0) {
-                    a.ml[u * 2] = mx;
-                    a.ml[u * 2 + 1] = sum;
-                }
-            }
+    float *lds = (float *)smem;
+    if (live) {
+        float *w = lds + (size_t)(32 * wave + l31) * LROW;
+#pragma unroll
+        for (int d = 0; d < DT; d++)
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                *(pf4_t *)(w + 32 * d + 8 * i + 4 * h) = pf4_t{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
+        const float l = l_run + __shfl_xor(l_run, 32, 64);
+        if (h == 0) {
+            w[D] = m_run;
+            w[D + 1] = l;
         }
     }
+    __syncthreads();
+    // thread t: a row, and its share of the channels
+    constexpr int TR = 512 / (32 * R), N = D / TR;
+    const int row = threadIdx.x / TR;
+    if (row < rows)
+        pg_join_row<D, N, KL>(a, it, kvh, row, (threadIdx.x % TR) * N, lds + (size_t)row * LROW, 32 * R * LROW, &bad_rows);
+    __syncthreads();
+    if (bad_rows) pg_rows_again<FMT, D>(a, it, kvh, lds);
 }
 
-// Partial results of a query joined; 4 channels a thread.  grid (queries, heads * D / 1024 rounded up)
+// Partial results of a query joined; 4 channels a thread.  Batches of U parts, so that
+// their loads are in flight together.  grid (queries, heads * D / 1024 rounded up)
 template <int D>
 __global__ __launch_bounds__(256) void k_pages_join(PageJoinArgs a) {
+    constexpr int U = 8;
     const PageJoin j = a.joins[blockIdx.x];
     const int e = blockIdx.y * 1024 + 4 * threadIdx.x;
     if (e >= a.heads * D) return;
-    const int hd = e / D;
+    const int hd = e / D, n = j.count;
     float mx = -INFINITY, l = 0.0f;
-    for (int i = 0; i < j.count; i++) mx = fmaxf(mx, a.ml[((size_t)a.units[j.first + i] * a.heads + hd) * 2]);
     pf4_t o = {0, 0, 0, 0};
-    for (int i = 0; i < j.count; i++) {
-        const size_t u = (size_t)a.units[j.first + i] * a.heads + hd;
-        const float mi = a.ml[u * 2], w = mi == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mi - mx);
-        l = __builtin_fmaf(a.ml[u * 2 + 1], w, l);
-        const pf4_t p = *(const pf4_t *)(a.part + u * D + e % D);
+    for (int i = 0; i < n; i += U) {
+        float mi[U], li[U];
+        pf4_t p[U];
 #pragma unroll
-        for (int k = 0; k < 4; k++) o[k] = __builtin_fmaf(p[k], w, o[k]);
+        for (int k = 0; k < U; k++) {
+            const size_t u = (size_t)a.units[j.first + min(i + k, n - 1)] * a.heads + hd;
+            mi[k] = a.ml[u * 2];
+            li[k] = a.ml[u * 2 + 1];
+            p[k] = *(const pf4_t *)(a.part + u * D + e % D);
+        }
+        float mn = mx;
+#pragma unroll
+        for (int k = 0; k < U; k++) mn = fmaxf(mn, mi[k]);
+        const float al = mx == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mx - mn);
+        mx = mn;
+        l *= al;
+#pragma unroll
+        for (int c = 0; c < 4; c++) o[c] *= al;
+#pragma unroll
+        for (int k = 0; k < U; k++) {
+            if (i + k >= n) break;
+            const float w = mi[k] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mi[k] - mx);
+            l = __builtin_fmaf(li[k], w, l);
+#pragma unroll
+            for (int c = 0; c < 4; c++) o[c] = __builtin_fmaf(p[k][c], w, o[c]);
+        }
     }
-    const float il = j.count ? 1.0f / l : 0.0f;
+    const float il = n ? 1.0f / l : 0.0f;
 #pragma unroll
     for (int k = 0; k < 4; k++) o[k] *= il;
     *(pf4_t *)(a.out + (size_t)j.query * a.heads * D + e) = o;
 }
 
 // f32 rows into their slots: a thread takes 32 channels of K or V of one token,
-// layer and kv head (as fl_kv_write's Q8 writer, its arithmetic)
+// layer and kv head
 template <int FMT, int D>
-__global__ __launch_bounds__(256) void k_pages_write(PageWriteArgs a) {
+__global__ __launch_bounds__(256) void k_pages_write(PageWriteArgs a, PageSlots slots) {
     constexpr int NB = D / 32;
     const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
     const long long total = (long long)a.layers * a.n * a.pool.nkv * NB * 2;
@@ -541,7 +757,7 @@ __global__ __launch_bounds__(256) void k_pages_write(PageWriteArgs a) {
     const int kvh = (int)(j % a.pool.nkv);
     j /= a.pool.nkv;
     const int t = (int)(j % a.n), l = (int)(j / a.n);
-    const int at = a.slots[t], page = at / a.pool.P, slot = at % a.pool.P;
+    const int at = slots.list ? slots.list[t] : slots.some[t], page = at / a.pool.P, slot = at % a.pool.P;
     const float *x = (isv ? a.v : a.k) + ((long long)l * a.n + t) * a.stride + kvh * D + 32 * b;
     const size_t head = ((size_t)(a.layer0 + l) * a.pool.pages + page) * a.pool.nkv + kvh;
     const size_t base = isv ? head * a.pool.P * D + ((size_t)(slot >> 5) * D + 32 * b) * 32 + (slot & 31)
@@ -551,8 +767,8 @@ __global__ __launch_bounds__(256) void k_pages_write(PageWriteArgs a) {
     if constexpr (FMT == FL_KV_Q8) {
         float amax = 0.0f;
         for (int e = 0; e < 32; e++) amax = fmaxf(amax, fabsf(x[e]));
-        const float d = amax / 127.0f;
-        const float id = (d != 0.0f) ? 127.0f / amax : 0.0f;
+        float d, id;
+        pg_q8_scale(amax, d, id);
         for (int e = 0; e < 32; e++) ((int8_t *)o)[base + (size_t)e * step] = q8_code(x[e] * id);
         (isv ? a.pool.vs : a.pool.ks)[(head * a.pool.P + slot) * NB + b] = f2h(d);
     } else {
@@ -577,8 +793,8 @@ __global__ __launch_bounds__(256) void k_pages_read(PageReadArgs a) {
 
 // Blocks of pages to other pages: grid (copies, layers * kv heads); `unit` bytes of
 // a 32-slot block of K (and of V), `sunit` of its scales
-static __global__ __launch_bounds__(256) void k_pages_copy(PagePool p, const PageCopy *c, int unit, int sunit) {
-    const PageCopy x = c[blockIdx.x];
+static __global__ __launch_bounds__(256) void k_pages_copy(PagePool p, PageCopies c, int unit, int sunit) {
+    const PageCopy x = c.list ? c.list[blockIdx.x] : c.some[blockIdx.x];
     const int layer = blockIdx.y / p.nkv, kvh = blockIdx.y % p.nkv;
     const size_t per = p.P / kPageBlock;
     const size_t from = (((size_t)layer * p.pages + x.src) * p.nkv + kvh) * per;

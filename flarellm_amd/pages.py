@@ -13,7 +13,6 @@ torch operation; no call waits for the GPU.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
 
 import numpy as np
@@ -22,20 +21,15 @@ from . import _lib
 from ._lib import FL_KV_F16, FL_KV_F32, FL_KV_Q8, FlareError, PagesConfig, check
 
 
-def _ids(x, what: str) -> np.ndarray:
+def _ids(x, what: str, n: int = -1) -> np.ndarray:
     a = np.asarray(x)
-    if a.dtype == np.int32 and a.ndim == 1 and a.flags.c_contiguous:
-        return a
-    if a.ndim != 1 or (a.size and a.dtype.kind not in "iu"):
-        raise ValueError(f"{what}: a list of whole numbers")
-    if a.size and (a.max() > 2**31 - 1 or a.min() < -(2**31)):
-        raise ValueError(f"{what}: out of range")
-    return np.ascontiguousarray(a, np.int32)
-
-
-def _ids_of(n: int, x, what: str) -> np.ndarray:
-    a = _ids(x, what)
-    if a.size != n:
+    if a.dtype != np.int32 or a.ndim != 1:
+        if a.ndim != 1 or (a.size and a.dtype.kind not in "iu"):
+            raise ValueError(f"{what}: a list of whole numbers")
+        if a.size and (a.max() > 2**31 - 1 or a.min() < -(2**31)):
+            raise ValueError(f"{what}: out of range")
+        a = a.astype(np.int32)
+    if n >= 0 and a.size != n:
         raise ValueError(f"{what}: {a.size} values for {n} sequences")
     return a
 
@@ -68,6 +62,8 @@ class PagedKv:
                                                       dtype=torch.float16, device=self.device) for _ in "kv")
         #: the backend's stream: with it as the current one, calls need no events
         self.stream = torch.cuda.ExternalStream(backend.stream, device=self.device)
+        self._stream = self.stream.cuda_stream
+        self._row = (kv_heads, head_dim)
         # the memory may be what earlier work of the current stream still uses
         self.stream.wait_stream(torch.cuda.current_stream(self.device))
         h = C.c_void_p()
@@ -88,78 +84,81 @@ class PagedKv:
         except Exception:
             pass
 
-    def _call(self, name: str, *args):
+    def _call(self, fn, *args):
         if not self._h or not self._b.ctx:
             raise FlareError("the paged cache or its backend is closed")
-        check(getattr(self.lib, name)(self._h, *args), self._b.ctx)
+        rc = fn(self._h, *args)
+        if rc:
+            check(rc, self._b.ctx)
 
-    @contextlib.contextmanager
-    def _ordered(self):
-        """The current torch stream's work before this, and this before what follows there."""
+    def _enqueue(self, fn, *args):
+        """_call behind the current torch stream's work, and before what follows there."""
         import torch
 
+        current = torch._C._cuda_getCurrentRawStream(self.device.index)
+        if current == self._stream:
+            return self._call(fn, *args)
         current = torch.cuda.current_stream(self.device)
-        if current.cuda_stream == self.stream.cuda_stream:
-            yield
-            return
         self.stream.wait_stream(current)
-        yield
-        current.wait_stream(self.stream)
+        try:
+            self._call(fn, *args)
+        finally:
+            current.wait_stream(self.stream)
 
     def _rows(self, t, what: str, shape):
         """A float32 tensor on this device whose last dimensions are `shape`, without gaps between them."""
         import torch
 
-        if not torch.is_tensor(t) or t.dtype != torch.float32 or t.device != self.device:
+        if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.device != self.device:
             raise ValueError(f"{what}: a float32 tensor on {self.device}")
         n = len(shape)
-        if t.dim() < n or tuple(t.shape[-n:]) != tuple(shape):
+        if t.shape[-n:] != shape:
             raise ValueError(f"{what}: {tuple(t.shape)}, not [.., {', '.join(map(str, shape))}]")
+        if t.is_contiguous():
+            return
         want = 1
-        for size, stride in zip(reversed(t.shape[-n:]), reversed(t.stride()[-n:])):
+        for size, stride in zip(reversed(shape), reversed(t.stride()[-n:])):
             if size != 1 and stride != want:
                 raise ValueError(f"{what}: gaps within a row")
             want *= size
 
     # ---- sequences ----------------------------------------------------------
+    # (lists go to the library as bytes: their address is the cheapest that numpy gives)
     def fork(self, src, dst, lens=None):
         """dst[i] (empty) becomes the first lens[i] tokens (all of them) of src[i], on the same pages."""
         src = _ids(src, "src")
-        dst = _ids_of(len(src), dst, "dst")
-        lens = None if lens is None else _ids_of(len(src), lens, "lens")
-        self._call("fl_pages_fork", src.ctypes.data, dst.ctypes.data, None if lens is None else lens.ctypes.data, len(src))
+        n = src.size
+        dst = _ids(dst, "dst", n)
+        lens = None if lens is None else _ids(lens, "lens", n).tobytes()
+        self._call(self.lib.fl_pages_fork, src.tobytes(), dst.tobytes(), lens, n)
 
     def copy(self, src, dst):
         """dst[i] (empty) becomes a copy of src[i] on pages of its own."""
         src = _ids(src, "src")
-        dst = _ids_of(len(src), dst, "dst")
-        with self._ordered():
-            self._call("fl_pages_copy", src.ctypes.data, dst.ctypes.data, len(src))
+        dst = _ids(dst, "dst", src.size)
+        self._enqueue(self.lib.fl_pages_copy, src.tobytes(), dst.tobytes(), src.size)
 
     def free(self, seqs):
         """Empties sequences; pages that none holds any more are free."""
         seqs = _ids(seqs, "seqs")
-        self._call("fl_pages_free", seqs.ctypes.data, len(seqs))
+        self._call(self.lib.fl_pages_free, seqs.tobytes(), seqs.size)
 
     def truncate(self, seqs, lens):
         """Cuts sequences to their first lens[i] tokens."""
         seqs = _ids(seqs, "seqs")
-        lens = _ids_of(len(seqs), lens, "lens")
-        self._call("fl_pages_truncate", seqs.ctypes.data, lens.ctypes.data, len(seqs))
+        lens = _ids(lens, "lens", seqs.size)
+        self._call(self.lib.fl_pages_truncate, seqs.tobytes(), lens.tobytes(), seqs.size)
 
     def extend(self, seqs, counts):
         """Reserves slots for counts[i] more tokens of each sequence; `write` fills them, layer by layer."""
         seqs = _ids(seqs, "seqs")
-        counts = _ids_of(len(seqs), counts, "counts")
-        with self._ordered():
-            self._call("fl_pages_extend", seqs.ctypes.data, counts.ctypes.data, len(seqs))
-        self._tokens = int(counts.sum())
+        counts = _ids(counts, "counts", seqs.size)
+        self._enqueue(self.lib.fl_pages_extend, seqs.tobytes(), counts.tobytes(), seqs.size)
 
     def compact(self) -> int:
         """Moves pages so that those in use have the lowest numbers; returns how many moved."""
         n = C.c_int()
-        with self._ordered():
-            self._call("fl_pages_compact", C.byref(n))
+        self._enqueue(self.lib.fl_pages_compact, C.byref(n))
         return n.value
 
     def length(self, seq: int) -> int:
@@ -175,12 +174,12 @@ class PagedKv:
     def tables(self) -> np.ndarray:
         """Page lists [max_seqs, pages of max_len], -1 where a sequence holds none."""
         t = np.empty((self.max_seqs, -(-self.max_len // self.page_size)), np.int32)
-        self._call("fl_pages_tables", t.ctypes.data, None)
+        self._call(self.lib.fl_pages_tables, t.ctypes.data, None)
         return t
 
     def lens(self) -> np.ndarray:
         n = np.empty(self.max_seqs, np.int32)
-        self._call("fl_pages_tables", None, n.ctypes.data)
+        self._call(self.lib.fl_pages_tables, None, n.ctypes.data)
         return n
 
     # ---- rows ---------------------------------------------------------------
@@ -188,34 +187,32 @@ class PagedKv:
         """Keys and values of the last `extend`'s tokens, sequence by sequence: [tokens, kv_heads, head_dim]
         for one layer, or [layers, tokens, kv_heads, head_dim] for as many from `layer` on.  Token rows
         may be slices of wider ones."""
-        row = (self.kv_heads, self.head_dim)
-        for t, what in ((k, "k"), (v, "v")):
-            self._rows(t, what, row)
+        self._rows(k, "k", self._row)
+        self._rows(v, "v", self._row)
         if k.dim() not in (3, 4) or k.shape != v.shape or k.stride() != v.stride():
             raise ValueError("k and v: [tokens, kv_heads, head_dim] or [layers, ..], laid out alike")
         n = k.shape[-3]
-        if n != getattr(self, "_tokens", -1):
-            raise ValueError(f"{n} tokens, where the last extend() made room for {getattr(self, '_tokens', 0)}")
+        room = self.lib.fl_pages_pending(self._h) if self._h else n
+        if room >= 0 and n != room:
+            raise ValueError(f"{n} tokens, where the last extend() made room for {room}")
         if n == 0:
             return
         layers = k.shape[0] if k.dim() == 4 else 1
         stride = k.stride(-3) if n > 1 else max(k.stride(-3), self.kv_heads * self.head_dim)
         if layers > 1 and k.stride(0) != n * stride:
             raise ValueError("k and v: gaps between layers")
-        with self._ordered():
-            self._call("fl_pages_write", layer, layers, k.data_ptr(), v.data_ptr(), stride)
+        self._enqueue(self.lib.fl_pages_write, layer, layers, k.data_ptr(), v.data_ptr(), stride)
 
     def read(self, seqs, starts, counts, layer: int = 0):
         """The f32 keys and values [tokens, kv_heads, head_dim] of counts[i] tokens of each sequence, from starts[i] on."""
         import torch
 
         seqs = _ids(seqs, "seqs")
-        starts, counts = _ids_of(len(seqs), starts, "starts"), _ids_of(len(seqs), counts, "counts")
+        starts, counts = _ids(starts, "starts", seqs.size), _ids(counts, "counts", seqs.size)
         shape = (max(0, int(counts.sum())), self.kv_heads, self.head_dim)
         k, v = (torch.empty(shape, dtype=torch.float32, device=self.device) for _ in "kv")
-        with self._ordered():
-            self._call("fl_pages_read", layer, seqs.ctypes.data, starts.ctypes.data, counts.ctypes.data, len(seqs),
-                       k.data_ptr(), v.data_ptr())
+        self._enqueue(self.lib.fl_pages_read, layer, seqs.tobytes(), starts.tobytes(), counts.tobytes(), seqs.size,
+                      k.data_ptr(), v.data_ptr())
         return k, v
 
     def attention(self, q, seqs, seen=None, layer: int = 0, out=None):
@@ -223,24 +220,23 @@ class PagedKv:
         over the first seen[i] tokens (all of them) of sequence seqs[i].  -> [n, heads, head_dim]"""
         import torch
 
-        if not torch.is_tensor(q) or q.dim() != 3:
+        if not isinstance(q, torch.Tensor) or q.dim() != 3:
             raise ValueError("q: [n, heads, head_dim]")
-        n, heads, _ = q.shape
+        n, heads, _ = shape = q.shape
         self._rows(q, "q", (heads, self.head_dim))
-        seqs = _ids_of(n, seqs, "seqs")
+        seqs = _ids(seqs, "seqs", n)
         if seen is None:
             if n and (seqs.min() < 0 or seqs.max() >= self.max_seqs):
                 raise ValueError(f"seqs: of {self.max_seqs}")
             seen = self.lens()[seqs]
-        seen = _ids_of(n, seen, "seen")
+        seen = _ids(seen, "seen", n)
         if out is None:
-            out = torch.empty(n, heads, self.head_dim, dtype=torch.float32, device=self.device)
+            out = torch.empty(shape, dtype=torch.float32, device=self.device)
         else:
-            self._rows(out, "out", (n, heads, self.head_dim))
+            self._rows(out, "out", shape)
             if out.dim() != 3:
                 raise ValueError("out: [n, heads, head_dim]")
         stride = q.stride(0) if n > 1 else max(q.stride(0), heads * self.head_dim)
-        with self._ordered():
-            self._call("fl_pages_attention", layer, q.data_ptr(), stride, seqs.ctypes.data, seen.ctypes.data, n, heads,
-                       out.data_ptr())
+        self._enqueue(self.lib.fl_pages_attention, layer, q.data_ptr(), stride, seqs.tobytes(), seen.tobytes(), n, heads,
+                      out.data_ptr())
         return out

@@ -378,7 +378,8 @@ int fl_read_tokens(fl_ctx *ctx, int start, int n, uint32_t *out);
  * fl_pages_bytes):
  *   k [layer][page][kv head][slot][head_dim]
  *   v [layer][page][kv head][slot / 32][head_dim][32]
- * f32, binary16, or int8 codes with a binary16 scale per 32 channels:
+ * f32, binary16, or int8 codes with a binary16 scale per 32 channels (amax * (1 /
+ * 127); codes x * (1 / amax * 127), halves away from zero):
  *   k_scale, v_scale [layer][page][kv head][slot][head_dim / 32]   (FL_KV_Q8)
  *
  * The bookkeeping is the host's and immediate.  Every call checks its arguments
@@ -438,8 +439,10 @@ int fl_pages_read(fl_pages *p, int layer, const int32_t *seqs, const int32_t *st
  * [n][num_heads * head_dim] f32, 16-byte aligned.  Up to 32 query heads per kv head. */
 int fl_pages_attention(fl_pages *p, int layer, const float *q, size_t q_stride, const int32_t *seqs,
                        const int32_t *seen, int n, int num_heads, float *out);
-/* Tokens of a sequence, free pages of the pool (-1: no such). */
+/* Tokens of a sequence, tokens that fl_pages_write stores, free pages of the pool
+ * (-1: no such sequence, nothing to write for). */
 int fl_pages_len(const fl_pages *p, int seq);
+int fl_pages_pending(const fl_pages *p);
 int fl_pages_free_count(const fl_pages *p);
 /* All page lists [max_seqs][max_seq_len / page_size rounded up] (-1 where a
  * sequence holds none) and all lengths (either may be NULL). */

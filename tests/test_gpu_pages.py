@@ -29,10 +29,10 @@ def stored(fmt, x):
         return x.astype(np.float16).astype(np.float32)
     b = x.reshape(-1, 32)
     amax = np.abs(b).max(1, keepdims=True)
-    inv = np.where(amax > 0, np.float32(127.0) / np.where(amax > 0, amax, 1).astype(np.float32), np.float32(0))
+    inv = np.where(amax > 0, np.float32(1) / np.where(amax > 0, amax, np.float32(1)) * np.float32(127), np.float32(0))
     y = (b * inv).astype(np.float32)
     code = np.trunc(y + np.copysign(np.float32(0.49999997), y))
-    scale = (amax / np.float32(127.0)).astype(np.float16).astype(np.float32)
+    scale = (amax * (np.float32(1) / np.float32(127))).astype(np.float16).astype(np.float32)
     return (code * scale).astype(np.float32).reshape(x.shape)
 
 
