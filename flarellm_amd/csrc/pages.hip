@@ -509,7 +509,7 @@ int fl_pages_attention(fl_pages *p, int layer, const float *q, size_t q_stride, 
     }
     if (!l.joins.empty()) {
         PageJoinArgs j{(const PageJoin *)(d + p->plan_joins), (const int *)(d + p->plan_units), a.part, a.ml, out, num_heads};
-        const dim3 grid((unsigned)l.joins.size(), (unsigned)((num_heads * D + 1023) / 1024));
+        const dim3 grid((unsigned)l.joins.size(), (unsigned)((num_heads * D + 127) / 128));
         if (D == 64) hipLaunchKernelGGL(k_pages_join<64>, grid, dim3(256), 0, p->stream, j);
         else hipLaunchKernelGGL(k_pages_join<128>, grid, dim3(256), 0, p->stream, j);
         PGCHK(p, hipGetLastError());

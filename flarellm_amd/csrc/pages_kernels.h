@@ -26,8 +26,13 @@ __device__ __forceinline__ void pg_split(const float *x, pu4_t &hi, pu4_t &lo) {
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         const auto h = __builtin_amdgcn_cvt_pkrtz(x[2 * i], x[2 * i + 1]);
-        const auto l = __builtin_amdgcn_cvt_pkrtz(x[2 * i] - (float)h[0], x[2 * i + 1] - (float)h[1]);
         hi[i] = __builtin_bit_cast(uint32_t, h);
+        // x minus its high part, exactly, in one instruction each (a conversion and a
+        // subtraction otherwise)
+        float a, b;
+        asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(a) : "v"(hi[i]), "v"(x[2 * i]));
+        asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(b) : "v"(hi[i]), "v"(x[2 * i + 1]));
+        const auto l = __builtin_amdgcn_cvt_pkrtz(a, b);
         lo[i] = __builtin_bit_cast(uint32_t, l);
     }
 }
@@ -497,13 +502,12 @@ __global__ __launch_bounds__(256) void k_pages_attn(PageAttnArgs a) {
 #pragma unroll
                     for (int i = 0; i < 4; i++) o[n][d][i] *= al;
             }
-            // a row that has seen no token yet keeps p = 0
+            // (a row that has seen no token yet has scores of -Inf alone, and p = 0)
             const float off = m_run[n] == -INFINITY ? -INFINITY : kPageShift<FMT> - m_run[n];
             float p[8];
 #pragma unroll
             for (int j = 0; j < 8; j++) {
-                const float y = s[n][j >> 2][j & 3];
-                p[j] = y == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(__builtin_fmaf(y, c[n], off));
+                p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][j >> 2][j & 3], c[n], off));
                 l_run[n] += p[j];
             }
             blk.add_pv(p, g, o[n]);
@@ -560,7 +564,11 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 
     // chunk p (16 B) of a K block in LDS holds chunk c ^ g(row) of its row, g from row bits
     // 0, 1, 3 (the rows that 8 lanes read together differ in those); of a V block, chunk
-    // c ^ (channel >> 1 & 3) of its channel
+    // c ^ (channel >> 1 & 3) of its channel.  A copy of 64 chunks: the lane's place among
+    // them, but for row bit 3, which is a bit of the copy's number.
+    const int r8 = lane / CH;
+    const int place = 16 * (wave < 4 ? r8 * CH + ((lane % CH) ^ (r8 & 3)) : (lane & ~3) | ((lane & 3) ^ ((lane >> 3) & 3)));
+    const int flip = wave < 4 ? 64 : 0;
     auto copy = [&](int step, int buf) {
         const int w = wave & 3, b = min(4 * step + w, nb - 1), tok = it.slot0 + 32 * b;
         const int page = __builtin_amdgcn_readfirstlane(a.page_ids[it.page0 + tok / P - it.slot0 / P]);
@@ -568,11 +576,8 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         const char *src = (const char *)(wave < 4 ? a.pool.k : a.pool.v) + at;
         char *dst = smem + (size_t)(8 * buf + wave) * BLK;
 #pragma unroll
-        for (int u = 0; u < BLK / 1024; u++) {
-            const int p = 64 * u + lane, r = p / CH, g = (r & 3) | ((r >> 1) & 4);
-            const int off = wave < 4 ? r * CH + ((p % CH) ^ g) : (p & ~3) | ((p & 3) ^ ((p >> 3) & 3));
-            copy_to_lds(src + off * 16, dst + u * 1024);
-        }
+        for (int u = 0; u < BLK / 1024; u++)
+            copy_to_lds(src + u * 1024 + (((u * 64 / CH) & 8) ? place ^ flip : place), dst + u * 1024);
     };
     copy(0, 0);
 
@@ -600,6 +605,12 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     float m_run = -INFINITY, l_run = 0.0f;
     const int krow = (l31 & 0x13) | ((l31 & 4) << 1) | ((l31 & 8) >> 1);
     const int kg = (krow & 3) | ((krow >> 1) & 4);
+    // of its K row, chunk 2 k + h: 4 places, and those 128 B behind; of a V block, chunk 2 mm + h of channel l31
+    int kat[4], vat[2];
+#pragma unroll
+    for (int k = 0; k < 4; k++) kat[k] = krow * D * 2 + (((2 * k + h) ^ kg) * 16);
+#pragma unroll
+    for (int mm = 0; mm < 2; mm++) vat[mm] = l31 * 64 + (((2 * mm + h) ^ ((l31 >> 1) & 3)) * 16);
 
     for (int step = 0; step < nit; step++) {
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
@@ -618,20 +629,30 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
             __syncthreads();
         }
         if (!live) continue;
-#pragma unroll 1
+        // Operands are read from LDS a phase ahead: V before the softmax, the next
+        // block's K before the products with V.
+        pu4_t kf[KS], vf[DT][2];
+        auto load_k = [&](int bi) {
+            const char *kt = smem + (size_t)(8 * buf + bi) * BLK;
+#pragma unroll
+            for (int k = 0; k < KS; k++) kf[k] = *(const pu4_t *)(kt + kat[k & 3] + (k >> 2) * 128);
+        };
+        load_k(NB * kl);
+#pragma unroll
         for (int i = 0; i < NB; i++) {
             const int bi = NB * kl + i, tok = it.slot0 + 32 * (4 * step + bi);
             if (tok >= it.slot1) break;
-            const char *kt = smem + (size_t)(8 * buf + bi) * BLK + krow * D * 2, *vt = smem + (size_t)(8 * buf + 4 + bi) * BLK;
-            pf16_t s = zero, lo = zero;
+            pf16_t s = zero;
 #pragma unroll
-            for (int k = 0; k < KS; k++) {
-                const pu4_t kf = *(const pu4_t *)(kt + (((2 * k + h) ^ kg) * 16));
-                lo = pg_mfma_w(kf, q[k][1], lo);
-                s = pg_mfma_w(kf, q[k][0], s);
-            }
+            for (int k = 0; k < KS; k++) s = pg_mfma_w(kf[k], q[k][1], s);
 #pragma unroll
-            for (int j = 0; j < 16; j++) s[j] += lo[j];
+            for (int k = 0; k < KS; k++) s = pg_mfma_w(kf[k], q[k][0], s);
+            const char *vt = smem + (size_t)(8 * buf + 4 + bi) * BLK;
+#pragma unroll
+            for (int d = 0; d < DT; d++)
+#pragma unroll
+                for (int mm = 0; mm < 2; mm++) vf[d][mm] = *(const pu4_t *)(vt + vat[mm] + d * 2048);
+            __builtin_amdgcn_sched_barrier(0);
             if (tok + 32 > it.smin) {  // some query does not see every token
                 const int end = min(pq.seen, it.slot1) - tok;
 #pragma unroll
@@ -652,27 +673,25 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 #pragma unroll
                     for (int j = 0; j < 16; j++) o[d][j] *= al;
             }
-            // a row that has seen no token yet keeps p = 0 (a score of -Inf makes the exponent -Inf, too)
+            // (a row that has seen no token yet has scores of -Inf alone, and p = 0)
             const float off = m_run == -INFINITY ? -INFINITY : kPageShift<FMT> - m_run;
             float p[16];
 #pragma unroll
             for (int j = 0; j < 16; j++) {
-                p[j] = __builtin_amdgcn_exp2f(s[j] == -INFINITY ? -INFINITY : __builtin_fmaf(s[j], c, off));
+                p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j], c, off));
                 l_run += p[j];
             }
             pu4_t pf[2][2];
             pg_split(p, pf[0][0], pf[0][1]);
             pg_split(p + 8, pf[1][0], pf[1][1]);
+            if (i + 1 < NB) load_k(bi + 1);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int d = 0; d < DT; d++) {
-                const int dd = 32 * d + l31;
+            for (int mm = 0; mm < 2; mm++)
 #pragma unroll
-                for (int mm = 0; mm < 2; mm++) {
-                    const pu4_t vf = *(const pu4_t *)(vt + dd * 64 + (((2 * mm + h) ^ ((dd >> 1) & 3)) * 16));
-                    o[d] = pg_mfma_w(vf, pf[mm][1], o[d]);
-                    o[d] = pg_mfma_w(vf, pf[mm][0], o[d]);
-                }
-            }
+                for (int u = 1; u >= 0; u--)
+#pragma unroll
+                    for (int d = 0; d < DT; d++) o[d] = pg_mfma_w(vf[d][mm], pf[mm][u], o[d]);
         }
     }
     __syncthreads();
@@ -700,26 +719,28 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     if (bad_rows) pg_rows_again<FMT, D>(a, it, kvh, lds);
 }
 
-// Partial results of a query joined; 4 channels a thread.  Batches of U parts, so that
-// their loads are in flight together.  grid (queries, heads * D / 1024 rounded up)
+// Partial results of a query joined: a workgroup takes 128 channels, 4 a thread, and
+// 8 of its threads share each channel's parts (one thread for all of them took 25 us for
+// the 64 parts of a single query of 16384 tokens, so 4).  grid (queries, heads * D / 128)
 template <int D>
 __global__ __launch_bounds__(256) void k_pages_join(PageJoinArgs a) {
-    constexpr int U = 8;
+    constexpr int U = 4;
+    __shared__ __align__(16) float lds[8][32][4];
+    __shared__ float lml[8][32][2];
     const PageJoin j = a.joins[blockIdx.x];
-    const int e = blockIdx.y * 1024 + 4 * threadIdx.x;
-    if (e >= a.heads * D) return;
-    const int hd = e / D, n = j.count;
+    const int c = threadIdx.x & 31, s = threadIdx.x >> 5;
+    const int e = blockIdx.y * 128 + 4 * c, ec = min(e, a.heads * D - 4), hd = ec / D, n = j.count;
     float mx = -INFINITY, l = 0.0f;
     pf4_t o = {0, 0, 0, 0};
-    for (int i = 0; i < n; i += U) {
+    for (int i = s; i < n; i += 8 * U) {
         float mi[U], li[U];
         pf4_t p[U];
 #pragma unroll
         for (int k = 0; k < U; k++) {
-            const size_t u = (size_t)a.units[j.first + min(i + k, n - 1)] * a.heads + hd;
+            const size_t u = (size_t)a.units[j.first + min(i + 8 * k, n - 1)] * a.heads + hd;
             mi[k] = a.ml[u * 2];
             li[k] = a.ml[u * 2 + 1];
-            p[k] = *(const pf4_t *)(a.part + u * D + e % D);
+            p[k] = *(const pf4_t *)(a.part + u * D + ec % D);
         }
         float mn = mx;
 #pragma unroll
@@ -728,20 +749,33 @@ __global__ __launch_bounds__(256) void k_pages_join(PageJoinArgs a) {
         mx = mn;
         l *= al;
 #pragma unroll
-        for (int c = 0; c < 4; c++) o[c] *= al;
+        for (int k = 0; k < 4; k++) o[k] *= al;
 #pragma unroll
         for (int k = 0; k < U; k++) {
-            if (i + k >= n) break;
+            if (i + 8 * k >= n) break;
             const float w = mi[k] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mi[k] - mx);
             l = __builtin_fmaf(li[k], w, l);
 #pragma unroll
-            for (int c = 0; c < 4; c++) o[c] = __builtin_fmaf(p[k][c], w, o[c]);
+            for (int x = 0; x < 4; x++) o[x] = __builtin_fmaf(p[k][x], w, o[x]);
         }
     }
-    const float il = n ? 1.0f / l : 0.0f;
+    *(pf4_t *)lds[s][c] = o;
+    lml[s][c][0] = mx;
+    lml[s][c][1] = l;
+    __syncthreads();
+    if (s) return;
+    for (int i = 1; i < 8; i++) mx = fmaxf(mx, lml[i][c][0]);
+    float y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    l = 0.0f;
 #pragma unroll
-    for (int k = 0; k < 4; k++) o[k] *= il;
-    *(pf4_t *)(a.out + (size_t)j.query * a.heads * D + e) = o;
+    for (int i = 0; i < 8; i++) {
+        const float mi = lml[i][c][0], w = mi == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mi - mx);
+        l = __builtin_fmaf(lml[i][c][1], w, l);
+#pragma unroll
+        for (int x = 0; x < 4; x++) y[x] = __builtin_fmaf(lds[i][c][x], w, y[x]);
+    }
+    const float il = n ? 1.0f / l : 0.0f;
+    if (e < a.heads * D) *(pf4_t *)(a.out + (size_t)j.query * a.heads * D + e) = pf4_t{y[0] * il, y[1] * il, y[2] * il, y[3] * il};
 }
 
 // f32 rows into their slots: a thread takes 32 channels of K or V of one token,
