@@ -219,13 +219,16 @@ struct LaunchAttn {
     template <int FMT, int D>
     int operator()() const {
         const dim3 grid((unsigned)(items * a.pool.nkv));
-        if (form == 0) hipLaunchKernelGGL((k_pages_attn<FMT, D, 1>), grid, dim3(256), 0, st, a);
-        else if (form == 1) hipLaunchKernelGGL((k_pages_attn<FMT, D, 2>), grid, dim3(256), 0, st, a);
-        else if constexpr (FMT == FL_KV_F16) {
-            // two steps of K and V, or the waves' results
-            constexpr size_t lds = std::max(2 * 8 * 32 * D * 2, 8 * 32 * (D + 4) * 4);
-            if (form == 2) hipLaunchKernelGGL((k_pages_wide<D, 2>), grid, dim3(512), lds, st, a);
-            else hipLaunchKernelGGL((k_pages_wide<D, 4>), grid, dim3(512), lds, st, a);
+        if (form == 0) {
+            hipLaunchKernelGGL((k_pages_attn<FMT, D, 1>), grid, dim3(256), 0, st, a);
+        } else if constexpr (FMT == FL_KV_F16) {
+            // two steps of K and V, or one and the queries, or the waves' results
+            constexpr size_t row = (D + 4) * 4, kv = 8 * 32 * D * 2;
+            if (form == 1) hipLaunchKernelGGL((k_pages_wide<D, 1>), grid, dim3(256), std::max(2 * kv, 4 * 32 * row), st, a);
+            else if (form == 2) hipLaunchKernelGGL((k_pages_wide<D, 2>), grid, dim3(512), std::max(2 * kv, 8 * 32 * row), st, a);
+            else hipLaunchKernelGGL((k_pages_wide<D, 4>), grid, dim3(512), std::max(2 * kv, 8 * 32 * row), st, a);
+        } else {
+            hipLaunchKernelGGL((k_pages_attn<FMT, D, 2>), grid, dim3(256), 0, st, a);
         }
         return (int)hipGetLastError();
     }

@@ -98,9 +98,14 @@ __device__ __forceinline__ void pg_q8_scale(float amax, float &scale, float &fac
     factor = amax > 0.0f ? 1.0f / amax * 127.0f : 0.0f;
 }
 
-// p is kept times 2^15 where its parts are binary16, so that they hold 22 bits down to 2^-18
+// A row's O and sum are kept relative to a maximum that follows its scores only when one
+// is over it by 2^kPageLag (nearly every block has a new maximum of some row, and
+// bringing O to it is a third of a block's vector work).  p is kept times 2^kPageShift
+// where its parts are binary16: at most 2^15, and what its low part loses below 2^-24 is
+// 2^-33 of the largest p.
+constexpr float kPageLag = 6.0f;
 template <int FMT>
-constexpr float kPageShift = FMT == FL_KV_F32 ? 0.0f : 15.0f;
+constexpr float kPageShift = FMT == FL_KV_F32 ? 0.0f : 9.0f;
 
 // The operands of a 32-slot block of one (page, kv head), in registers.  Scores are
 // formed transposed, S^T = K Q^T, with 16 x 16 products: a query row is a lane (mod
@@ -354,9 +359,23 @@ __device__ __forceinline__ void pg_rows_again(const PageAttnArgs &a, const PageI
     }
 }
 
-// A row of an item's result: channels ch .. ch + N - 1 from the KL partial results at
+// An item's query rows into LDS, LROW floats apart (read from memory by the lanes that
+// need them, a load is 32 or 64 lines: 10 us of a 128-row item's prologue).
+template <int D, int LROW, int NTHR>
+__device__ __forceinline__ void pg_stage_q(const PageAttnArgs &a, const PageItem &it, int kvh, float *lds) {
+    constexpr int TR = D / 4;
+    const int G = a.group, rows = it.nq * G, c = threadIdx.x % TR * 4;
+#pragma unroll 4
+    for (int r = threadIdx.x / TR; r < rows; r += NTHR / TR) {
+        const int qi = r / G;
+        const float *src = a.q + a.order[it.q0 + qi].query * a.q_stride + (size_t)(kvh * G + r - qi * G) * D + c;
+        *(pf4_t *)(lds + r * LROW + c) = pf4_t{src[0], src[1], src[2], src[3]};
+    }
+}
+
+// A row of an item's result: channels ch .. ch + 3 from the KL partial results at
 // lds[i * step], each [D] O, max, sum.  Sets *bad where a value is not finite.
-template <int D, int N, int KL>
+template <int D, int KL>
 __device__ __forceinline__ void pg_join_row(const PageAttnArgs &a, const PageItem &it, int kvh, int row, int ch,
                                             const float *lds, int step, int *bad) {
     float mx = -INFINITY, sum = 0.0f, wt[KL];
@@ -373,22 +392,19 @@ __device__ __forceinline__ void pg_join_row(const PageAttnArgs &a, const PageIte
     const size_t u = (size_t)(it.unit < 0 ? a.order[it.q0 + qi].query : it.unit + qi) * nh + hd;
     float *op = (it.unit < 0 ? a.out : a.part) + u * D + ch;
     const float il = it.unit < 0 ? 1.0f / sum : 1.0f;
+    pf4_t y = {0, 0, 0, 0};
 #pragma unroll
-    for (int j = 0; j < N; j += 4) {
-        pf4_t y = {0, 0, 0, 0};
+    for (int i = 0; i < KL; i++) {
+        const pf4_t x = *(const pf4_t *)(lds + i * step + ch);
 #pragma unroll
-        for (int i = 0; i < KL; i++) {
-            const pf4_t x = *(const pf4_t *)(lds + i * step + ch + j);
-#pragma unroll
-            for (int k = 0; k < 4; k++) y[k] = __builtin_fmaf(x[k], wt[i], y[k]);
-        }
-#pragma unroll
-        for (int k = 0; k < 4; k++) {
-            y[k] *= il;
-            odd = __builtin_fmaf(y[k], 0.0f, odd);
-        }
-        *(pf4_t *)(op + j) = y;
+        for (int k = 0; k < 4; k++) y[k] = __builtin_fmaf(x[k], wt[i], y[k]);
     }
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        y[k] *= il;
+        odd = __builtin_fmaf(y[k], 0.0f, odd);
+    }
+    *(pf4_t *)op = y;
     if (it.unit >= 0 && ch == 0) {
         a.ml[u * 2] = mx;
         a.ml[u * 2 + 1] = sum;
@@ -438,15 +454,16 @@ __global__ __launch_bounds__(256) void k_pages_attn(PageAttnArgs a) {
     blk.load_k(a.pool, head, slot, m, g);
     blk.load_v(a.pool, head, slot, m, g);
 
+    pg_stage_q<D, LROW, 256>(a, it, kvh, lds);
+    __syncthreads();
     pu4_t q[NT][QP];
     float c[NT];
     int seen[NT];
 #pragma unroll
     for (int n = 0; n < NT; n++) {
-        const int r = min(16 * n + m, rows - 1), qi = r / G;
-        const PageQuery pq = a.order[it.q0 + qi];
-        seen[n] = pq.seen;
-        const float *qp = a.q + pq.query * a.q_stride + (size_t)(kvh * G + r % G) * D;
+        const int r = min(16 * n + m, rows - 1);
+        seen[n] = a.order[it.q0 + r / G].seen;
+        const float *qp = lds + r * LROW;
         c[n] = a.scale;
         float mul = 1.0f;
         if constexpr (FMT != FL_KV_F32) {
@@ -492,7 +509,7 @@ __global__ __launch_bounds__(256) void k_pages_attn(PageAttnArgs a) {
 #pragma unroll
             for (int j = 1; j < 8; j++) x = fmaxf(x, s[n][j >> 2][j & 3]);
             x = pg_max16(x) * c[n];
-            if (__any(x > m_run[n])) {
+            if (__any(x > m_run[n] + kPageLag)) {
                 const float mn = fmaxf(m_run[n], x);
                 const float al = m_run[n] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m_run[n] - mn);
                 m_run[n] = mn;
@@ -530,27 +547,28 @@ __global__ __launch_bounds__(256) void k_pages_attn(PageAttnArgs a) {
             w[D + 1] = l;
         }
         __syncthreads();
-        const int r = threadIdx.x >> 4, row = 16 * n + r;
-        if (row < rows)
-            pg_join_row<D, D / 16, 4>(a, it, kvh, row, (threadIdx.x & 15) * (D / 16), lds + r * LROW, 16 * LROW, &bad_rows);
+        for (int r = threadIdx.x / (D / 4); r < min(16, rows - 16 * n); r += 256 / (D / 4))
+            pg_join_row<D, 4>(a, it, kvh, 16 * n + r, threadIdx.x % (D / 4) * 4, lds + r * LROW, 16 * LROW, &bad_rows);
     }
     __syncthreads();
     if (bad_rows) pg_rows_again<FMT, D>(a, it, kvh, lds);
 }
 
-// Items of 33 to 32 R rows (R = 2, 4): 8 waves, R row groups of 32 x 8 / R key lanes.
-// A step is 128 tokens, K and V of its four 32-slot blocks copied memory -> LDS one step
-// ahead (wave w copies K or V of one block); a key lane takes R / 2 of them.  Products are
+// Items of up to 32 R rows: R row groups of 32 x 8 / R key lanes in 8 waves (R = 2, 4), or
+// one x 4 in 4 (R = 1).  A step is 128 tokens, K and V of its four 32-slot blocks copied
+// memory -> LDS one step ahead (of 8 waves, each copies K or V of one block, of 4 each
+// both of its own, and never waits for the others); a key lane takes one of them or two.  Products are
 // 32 x 32 x 16: a query row is a lane (mod 32), the K rows enter with index bits 2 and 3
 // swapped so that scores i = 8 mm + j of a lane are slots 16 mm + 8 (lane / 32) + j, the
 // operand of O^T = V^T P^T.  Bound by the matrix issue: 64 products of 32 cycles per block
 // and row group, two waves a SIMD, whose softmax runs beside the other's products.
 template <int D, int R>
-__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) void k_pages_wide(PageAttnArgs a) {
-    constexpr int FMT = FL_KV_F16, KL = 8 / R, NB = 4 / KL;
+__global__ __launch_bounds__(R == 1 ? 256 : 512) __attribute__((amdgpu_waves_per_eu(R == 1 ? 1 : 2, 2))) void k_pages_wide(
+    PageAttnArgs a) {
+    constexpr int FMT = FL_KV_F16, NW = R == 1 ? 4 : 8, KL = NW / R, NB = 4 / KL;
     constexpr int KS = D / 16, DT = D / 32, CH = D / 8, BLK = 32 * D * 2;  // BLK: bytes of a block's K (or V)
     constexpr int LROW = D + 4;
-    extern __shared__ __align__(16) char smem[];  // 2 x (4 K blocks, 4 V blocks); at the end [8 waves][32][LROW]
+    extern __shared__ __align__(16) char smem[];  // 2 x (4 K blocks, 4 V blocks); at the end [waves][32][LROW]
     __shared__ int bad_rows;
     const int lane = threadIdx.x & 63, l31 = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), rg = wave % R, kl = wave / R;
@@ -567,23 +585,32 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     // c ^ (channel >> 1 & 3) of its channel.  A copy of 64 chunks: the lane's place among
     // them, but for row bit 3, which is a bit of the copy's number.
     const int r8 = lane / CH;
-    const int place = 16 * (wave < 4 ? r8 * CH + ((lane % CH) ^ (r8 & 3)) : (lane & ~3) | ((lane & 3) ^ ((lane >> 3) & 3)));
-    const int flip = wave < 4 ? 64 : 0;
+    const int kplace = 16 * (r8 * CH + ((lane % CH) ^ (r8 & 3))), vplace = 16 * ((lane & ~3) | ((lane & 3) ^ ((lane >> 3) & 3)));
     auto copy = [&](int step, int buf) {
         const int w = wave & 3, b = min(4 * step + w, nb - 1), tok = it.slot0 + 32 * b;
         const int page = __builtin_amdgcn_readfirstlane(a.page_ids[it.page0 + tok / P - it.slot0 / P]);
         const size_t at = (((layer_pages + page) * nkv + kvh) * P + tok % P) * D * 2;
-        const char *src = (const char *)(wave < 4 ? a.pool.k : a.pool.v) + at;
-        char *dst = smem + (size_t)(8 * buf + wave) * BLK;
+        char *dst = smem + (size_t)(8 * buf + w) * BLK;
+        if (R == 1 || wave < 4) {
 #pragma unroll
-        for (int u = 0; u < BLK / 1024; u++)
-            copy_to_lds(src + u * 1024 + (((u * 64 / CH) & 8) ? place ^ flip : place), dst + u * 1024);
+            for (int u = 0; u < BLK / 1024; u++)
+                copy_to_lds((const char *)a.pool.k + at + u * 1024 + (((u * 64 / CH) & 8) ? kplace ^ 64 : kplace), dst + u * 1024);
+        }
+        if (R == 1 || wave >= 4) {
+#pragma unroll
+            for (int u = 0; u < BLK / 1024; u++)
+                copy_to_lds((const char *)a.pool.v + at + u * 1024 + vplace, dst + 4 * BLK + u * 1024);
+        }
     };
     copy(0, 0);
 
+    // the queries, in the second buffer until its first copy
+    float *lds = (float *)smem, *ql = (float *)(smem + 8 * BLK);
+    pg_stage_q<D, LROW, 64 * NW>(a, it, kvh, ql);
+    __syncthreads();
     const int r0 = min(32 * rg + l31, rows - 1);
-    const PageQuery pq = a.order[it.q0 + r0 / G];
-    const float *qp = a.q + pq.query * a.q_stride + (size_t)(kvh * G + r0 % G) * D + 8 * h;
+    const int seen = a.order[it.q0 + r0 / G].seen;
+    const float *qp = ql + r0 * LROW + 8 * h;
     float c = a.scale, mul = 1.0f, x0 = 0.0f;
 #pragma unroll
     for (int k = 0; k < KS; k++)
@@ -598,6 +625,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         for (int j = 0; j < 8; j++) x[j] = qp[16 * k + j] * mul;
         pg_split(x, q[k][0], q[k][1]);
     }
+    if (R == 1) __syncthreads();  // (other waves' copies into the second buffer)
     const pf16_t zero = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
     pf16_t o[DT];
 #pragma unroll
@@ -614,23 +642,26 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 
     for (int step = 0; step < nit; step++) {
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-        __builtin_amdgcn_s_barrier();  // this step has landed, and nobody reads the other buffer
+        if (R > 1) __builtin_amdgcn_s_barrier();  // this step has landed, and nobody reads the other buffer
         asm volatile("" ::: "memory");
         const int buf = step & 1;
         if (step + 1 < nit) {
             copy(step + 1, buf ^ 1);
         } else if (const int over = (it.slot1 - it.slot0) & 31; over) {
             // slots behind the item's last token: whatever is there must not meet a zero
-            char *vb = smem + (size_t)(8 * buf + 4 + ((nb - 1) & 3)) * BLK;
-            for (int i = threadIdx.x; i < 32 * D; i += 512) {
-                const int d = i >> 5, s = i & 31;
-                if (s >= over) *(uint16_t *)(vb + d * 64 + (((s >> 3) ^ ((d >> 1) & 3)) * 16) + (s & 7) * 2) = 0;
-            }
-            __syncthreads();
+            const int lastb = (nb - 1) & 3;
+            char *vb = smem + (size_t)(8 * buf + 4 + lastb) * BLK;
+            if (R > 1 || wave == lastb)
+                for (int i = R > 1 ? threadIdx.x : lane; i < 32 * D; i += R > 1 ? 512 : 64) {
+                    const int d = i >> 5, s = i & 31;
+                    if (s >= over) *(uint16_t *)(vb + d * 64 + (((s >> 3) ^ ((d >> 1) & 3)) * 16) + (s & 7) * 2) = 0;
+                }
+            if (R > 1) __syncthreads();
+            else asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         }
         if (!live) continue;
         // Operands are read from LDS a phase ahead: V before the softmax, the next
-        // block's K before the products with V.
+        // block's K between the products with V.
         pu4_t kf[KS], vf[DT][2];
         auto load_k = [&](int bi) {
             const char *kt = smem + (size_t)(8 * buf + bi) * BLK;
@@ -654,7 +685,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
                 for (int mm = 0; mm < 2; mm++) vf[d][mm] = *(const pu4_t *)(vt + vat[mm] + d * 2048);
             __builtin_amdgcn_sched_barrier(0);
             if (tok + 32 > it.smin) {  // some query does not see every token
-                const int end = min(pq.seen, it.slot1) - tok;
+                const int end = min(seen, it.slot1) - tok;
 #pragma unroll
                 for (int j = 0; j < 16; j++)
                     if (16 * (j >> 3) + 8 * h + (j & 7) >= end) s[j] = -INFINITY;
@@ -663,7 +694,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 #pragma unroll
             for (int j = 1; j < 16; j++) m = fmaxf(m, s[j]);
             m = fmaxf(m, __shfl_xor(m, 32, 64)) * c;
-            if (__any(m > m_run)) {
+            if (__any(m > m_run + kPageLag)) {
                 const float mn = fmaxf(m_run, m);
                 const float al = m_run == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m_run - mn);
                 m_run = mn;
@@ -684,18 +715,21 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
             pu4_t pf[2][2];
             pg_split(p, pf[0][0], pf[0][1]);
             pg_split(p + 8, pf[1][0], pf[1][1]);
-            if (i + 1 < NB) load_k(bi + 1);
-            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int mm = 0; mm < 2; mm++)
+            for (int mm = 0; mm < 2; mm++) {
 #pragma unroll
                 for (int u = 1; u >= 0; u--)
 #pragma unroll
                     for (int d = 0; d < DT; d++) o[d] = pg_mfma_w(vf[d][mm], pf[mm][u], o[d]);
+                if (mm == 0) {
+                    __builtin_amdgcn_sched_barrier(0);
+                    if (i + 1 < NB) load_k(bi + 1);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
         }
     }
     __syncthreads();
-    float *lds = (float *)smem;
     if (live) {
         float *w = lds + (size_t)(32 * wave + l31) * LROW;
 #pragma unroll
@@ -710,11 +744,8 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         }
     }
     __syncthreads();
-    // thread t: a row, and its share of the channels
-    constexpr int TR = 512 / (32 * R), N = D / TR;
-    const int row = threadIdx.x / TR;
-    if (row < rows)
-        pg_join_row<D, N, KL>(a, it, kvh, row, (threadIdx.x % TR) * N, lds + (size_t)row * LROW, 32 * R * LROW, &bad_rows);
+    for (int r = threadIdx.x / (D / 4); r < rows; r += 64 * NW / (D / 4))
+        pg_join_row<D, KL>(a, it, kvh, r, threadIdx.x % (D / 4) * 4, lds + (size_t)r * LROW, 32 * R * LROW, &bad_rows);
     __syncthreads();
     if (bad_rows) pg_rows_again<FMT, D>(a, it, kvh, lds);
 }
