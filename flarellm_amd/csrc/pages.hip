@@ -23,6 +23,7 @@ struct Stage {
     bool used = false;
 };
 constexpr int kStages = 4;
+constexpr int kPageMaxGroup = 32;  // query heads per kv head: the rows of the largest form of every cache
 
 struct DevBuf {
     char *p = nullptr;
@@ -43,7 +44,7 @@ struct fl_pages {
     std::vector<int32_t> plan_seqs, plan_seen;
     int plan_heads = 0;
     uint64_t plan_version = 0;
-    size_t plan_items[kPageForms] = {}, plan_order = 0, plan_pages = 0, plan_units = 0, plan_joins = 0;  // offsets
+    size_t plan_order = 0, plan_pages = 0, plan_units = 0, plan_joins = 0;  // offsets
     DevBuf d_plan, d_slots, d_read, d_copies, ws;
     Stage stages[kStages];
     int stage = 0;
@@ -215,18 +216,18 @@ int with_form(int fmt, int D, F f) {
 struct LaunchAttn {
     hipStream_t st;
     const PageAttnArgs &a;
-    int items, form;
+    int items;
+    bool wide;
     template <int FMT, int D>
     int operator()() const {
         const dim3 grid((unsigned)(items * a.pool.nkv));
-        if (form == 0) {
+        if (!wide) {
             hipLaunchKernelGGL((k_pages_attn<FMT, D, 1>), grid, dim3(256), 0, st, a);
         } else if constexpr (FMT == FL_KV_F16) {
             // two steps of K and V, or one and the queries, or the waves' results
             constexpr size_t row = (D + 4) * 4, kv = 8 * 32 * D * 2;
-            if (form == 1) hipLaunchKernelGGL((k_pages_wide<D, 1>), grid, dim3(256), std::max(2 * kv, 4 * 32 * row), st, a);
-            else if (form == 2) hipLaunchKernelGGL((k_pages_wide<D, 2>), grid, dim3(512), std::max(2 * kv, 8 * 32 * row), st, a);
-            else hipLaunchKernelGGL((k_pages_wide<D, 4>), grid, dim3(512), std::max(2 * kv, 8 * 32 * row), st, a);
+            constexpr size_t lds = std::max({2 * kv, kv + 128 * row, 8 * 32 * row});
+            hipLaunchKernelGGL(k_pages_attn_wide<D>, grid, dim3(512), lds, st, a);
         } else {
             hipLaunchKernelGGL((k_pages_attn<FMT, D, 2>), grid, dim3(256), 0, st, a);
         }
@@ -257,7 +258,13 @@ struct LaunchRead {
     }
 };
 
-int forms_of(const fl_pages *p) { return p->cfg.kv_format == FL_KV_F16 ? 4 : 2; }
+// Costs fitted to measured calls (a block of 32 tokens of D = 128: 0.7 us where the memory
+// bounds it, 1.1 for 128 rows).
+const PageForms &forms_of(const fl_pages *p) {
+    static const PageForms f16 = {3, {16, 64, 128}, 768, {1, 1, 1.6f}, 6, 8, 256};
+    static const PageForms other = {2, {16, 32, 0}, 768, {2, 3, 0}, 6, 4, 512};
+    return p->cfg.kv_format == FL_KV_F16 ? f16 : other;
+}
 
 // The plan of these queries, on the device.
 int make_plan(fl_pages *p, const int32_t *seqs, const int32_t *seen, int n, int heads) {
@@ -267,7 +274,7 @@ int make_plan(fl_pages *p, const int32_t *seqs, const int32_t *seen, int n, int 
         return 0;
     p->plan_version = 0;
     PGTRY(on_table(p, [&](PageTable &t) {
-        const int rc = page_plan(t, seqs, seen, n, group, p->cfg.num_kv_heads, forms_of(p), p->plan);
+        const int rc = page_plan(t, seqs, seen, n, group, p->cfg.num_kv_heads, p->cfg.head_dim, forms_of(p), p->plan);
         if (rc) return rc;
         p->plan_seqs.assign(seqs, seqs + n);
         p->plan_seen.assign(seen, seen + n);
@@ -280,7 +287,7 @@ int make_plan(fl_pages *p, const int32_t *seqs, const int32_t *seen, int n, int 
         bytes = (bytes + b + 63) / 64 * 64;
         return at;
     };
-    for (int f = 0; f < kPageForms; f++) p->plan_items[f] = place(l.items[f].size() * sizeof(PageItem));
+    place(l.items.size() * sizeof(PageItem));
     p->plan_order = place(l.order.size() * sizeof(PageQuery));
     p->plan_pages = place(l.page_ids.size() * sizeof(int));
     p->plan_units = place(l.units.size() * sizeof(int));
@@ -292,7 +299,7 @@ int make_plan(fl_pages *p, const int32_t *seqs, const int32_t *seen, int n, int 
     auto put = [&](size_t at, const auto &v) {
         if (!v.empty()) memcpy(h + at, v.data(), v.size() * sizeof v[0]);
     };
-    for (int f = 0; f < kPageForms; f++) put(p->plan_items[f], l.items[f]);
+    put(0, l.items);
     put(p->plan_order, l.order);
     put(p->plan_pages, l.page_ids);
     put(p->plan_units, l.units);
@@ -482,7 +489,7 @@ int fl_pages_attention(fl_pages *p, int layer, const float *q, size_t q_stride, 
     PGTRY(check_layers(p, layer, 1));
     const int D = p->cfg.head_dim, nkv = p->cfg.num_kv_heads;
     if (num_heads < 1 || num_heads % nkv) return fail(p, FL_E_INVALID, "%d heads over %d kv heads", num_heads, nkv);
-    if (num_heads / nkv > kPageRows[1]) return fail(p, FL_E_UNSUPPORTED, "%d query heads per kv head", num_heads / nkv);
+    if (num_heads / nkv > kPageMaxGroup) return fail(p, FL_E_UNSUPPORTED, "%d query heads per kv head", num_heads / nkv);
     if (n < 0) return fail(p, FL_E_INVALID, "%d queries", n);
     if (n == 0) return 0;
     if (!q || !out || !seqs || !seen) return fail(p, FL_E_INVALID, "null argument");
@@ -505,11 +512,9 @@ int fl_pages_attention(fl_pages *p, int layer, const float *q, size_t q_stride, 
     a.part = (float *)p->ws.p;
     a.ml = a.part + (size_t)l.num_units * num_heads * D;
     a.out = out;
-    for (int f = kPageForms - 1; f >= 0; f--) {
-        if (l.items[f].empty()) continue;
-        a.items = (const PageItem *)(d + p->plan_items[f]);
-        PGCHK(p, (hipError_t)with_form(p->cfg.kv_format, D, LaunchAttn{p->stream, a, (int)l.items[f].size(), f}));
-    }
+    a.items = (const PageItem *)d;
+    if (!l.items.empty())
+        PGCHK(p, (hipError_t)with_form(p->cfg.kv_format, D, LaunchAttn{p->stream, a, (int)l.items.size(), l.wide}));
     if (!l.joins.empty()) {
         PageJoinArgs j{(const PageJoin *)(d + p->plan_joins), (const int *)(d + p->plan_units), a.part, a.ml, out, num_heads};
         const dim3 grid((unsigned)l.joins.size(), (unsigned)((num_heads * D + 127) / 128));
@@ -547,21 +552,20 @@ int fl_pages_copies(const fl_pages *p, int32_t *copies, int cap) {
 int fl_pages_plan(fl_pages *p, const int32_t *seqs, const int32_t *seen, int n, int num_heads, int32_t *items, int cap) {
     if (!p) return fail(p, FL_E_INVALID, "null pages");
     const int nkv = p->cfg.num_kv_heads;
-    if (num_heads < 1 || num_heads % nkv || num_heads / nkv > kPageRows[1])
+    if (num_heads < 1 || num_heads % nkv || num_heads / nkv > kPageMaxGroup)
         return fail(p, FL_E_INVALID, "%d heads over %d kv heads", num_heads, nkv);
     int made = 0;
     PGTRY(on_table(p, [&](PageTable &t) {
         PagePlan l;
-        const int rc = page_plan(t, seqs, seen, n, num_heads / nkv, nkv, forms_of(p), l);
+        const int rc = page_plan(t, seqs, seen, n, num_heads / nkv, nkv, p->cfg.head_dim, forms_of(p), l);
         if (rc) return rc;
-        for (int f = 0; f < kPageForms; f++)
-            for (const PageItem &it : l.items[f])
-                for (int i = 0; i < it.nq; i++, made++) {
-                    if (!items || made >= cap) continue;
-                    const int row[6] = {l.order[it.q0 + i].query, it.slot0, it.slot1, l.page_ids[it.page0], f,
-                                        it.unit < 0 ? -1 : it.unit + i};
-                    memcpy(items + 6 * made, row, sizeof row);
-                }
+        for (const PageItem &it : l.items)
+            for (int i = 0; i < it.nq; i++, made++) {
+                if (!items || made >= cap) continue;
+                const int row[6] = {l.order[it.q0 + i].query, it.slot0, it.slot1, l.page_ids[it.page0], it.form,
+                                    it.unit < 0 ? -1 : it.unit + i};
+                memcpy(items + 6 * made, row, sizeof row);
+            }
         return 0;
     }));
     return made;

@@ -3,8 +3,10 @@
 
 #include <algorithm>
 #include <climits>
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
+#include <functional>
 #include <numeric>
 
 namespace fl {
@@ -242,11 +244,11 @@ int PageTable::compact() {
 // the same sequences hold, as long as it can be: it ends where two of them
 // differ, not where one of them ends (its queries are masked there).  So each page
 // is in one run per set of sequences that hold it, and is read once for all of
-// them.  A run's queries, longest first, are cut into tiles of up to 32 rows (query
-// x head of a kv head) and its tokens into parts, until the chip is full.
+// them.  A run's queries, longest first, are cut into tiles by the rows (query x head of a
+// kv head) that a form takes, and its tokens into parts.
 // ---------------------------------------------------------------------------
-int page_plan(PageTable &t, const int32_t *s, const int32_t *seen, int n, int group, int kv_heads, int forms,
-              PagePlan &p) {
+int page_plan(PageTable &t, const int32_t *s, const int32_t *seen, int n, int group, int kv_heads,
+              int head_dim, const PageForms &forms, PagePlan &p) {
     auto fail = [&](int code, const std::string &m) {
         t.error = m;
         return code;
@@ -259,7 +261,7 @@ int page_plan(PageTable &t, const int32_t *s, const int32_t *seen, int n, int gr
             return fail(FL_E_INVALID, "query " + std::to_string(i) + " sees " + std::to_string(seen[i]) + " of " +
                                           std::to_string(t.len[s[i]]) + " tokens");
     }
-    for (auto &v : p.items) v.clear();
+    p.items.clear();
     p.order.clear();
     p.page_ids.clear();
     p.units.clear();
@@ -284,23 +286,44 @@ int page_plan(PageTable &t, const int32_t *s, const int32_t *seen, int n, int gr
             seqs.push_back({t.row(s[by[i]]), ceil_div(seen[by[i]], P), i, 1});
         }
     }
-    // a list that ends is behind those that go on
-    std::sort(seqs.begin(), seqs.end(), [](const Seq &a, const Seq &b) {
-        const int m = std::min(a.held, b.held);
-        const int k = (int)(std::mismatch(a.pages, a.pages + m, b.pages).first - a.pages);
-        if (k < m) return a.pages[k] < b.pages[k];
-        return a.held != b.held ? a.held > b.held : a.first < b.first;
-    });
-
     struct Run {
         int lo, hi, p0, p1;  // sequences, pages
     };
     struct Tile {
         int q0, nq, slot0, slot1, page0, form;
     };
-    std::vector<Run> todo{{0, (int)seqs.size(), 0, 0}};
+    std::vector<Run> todo;
     std::vector<Tile> tiles;
-    const int most = std::max(1, kPageRows[forms - 1] / group);  // queries of the largest tile
+    const int most = std::max(1, forms.rows[forms.n - 1] / group);  // queries of the largest tile
+    auto add_tile = [&](int q0, int nq, int from, int end, int page0) {
+        int form = 0;
+        while (forms.rows[form] < nq * group) form++;
+        tiles.push_back({q0, nq, from, std::min(p.order[q0].seen, end), page0, form});
+    };
+    // A sequence with enough queries for the largest tile: full tiles of its own, over all
+    // that they see (they gain nothing from others' queries, and need no joining).
+    for (Seq &x : seqs) {
+        const int full = x.count / most;
+        if (!full || !seen[by[x.first]]) continue;
+        const int page0 = (int)p.page_ids.size();
+        p.page_ids.insert(p.page_ids.end(), x.pages, x.pages + x.held);
+        for (int i = 0; i < full && seen[by[x.first]]; i++) {
+            const int q0 = (int)p.order.size();
+            for (int j = 0; j < most && seen[by[x.first]]; j++, x.first++, x.count--)
+                p.order.push_back({by[x.first], seen[by[x.first]]});
+            add_tile(q0, (int)p.order.size() - q0, 0, t.max_len, page0);
+            if (!x.count) break;
+        }
+        x.held = x.count ? ceil_div(seen[by[x.first]], P) : 0;
+    }
+    // the others: a list that ends is behind those that go on
+    std::sort(seqs.begin(), seqs.end(), [](const Seq &a, const Seq &b) {
+        const int m = std::min(a.held, b.held);
+        const int k = (int)(std::mismatch(a.pages, a.pages + m, b.pages).first - a.pages);
+        if (k < m) return a.pages[k] < b.pages[k];
+        return a.held != b.held ? a.held > b.held : a.first < b.first;
+    });
+    todo.push_back({0, (int)seqs.size(), 0, 0});
     while (!todo.empty()) {
         Run r = todo.back();
         todo.pop_back();
@@ -335,43 +358,84 @@ int page_plan(PageTable &t, const int32_t *s, const int32_t *seen, int n, int gr
         });
         const int page0 = (int)p.page_ids.size();
         for (int i = r.p0; i < e; i++) p.page_ids.push_back(seqs[r.lo].pages[i]);
-        for (int i = 0; i < total; i += most) {
-            const int nq = std::min(most, total - i);
-            int form = 0;
-            while (kPageRows[form] < nq * group) form++;
-            tiles.push_back({first + i, nq, from, std::min(p.order[first + i].seen, end), page0, form});
-        }
+        for (int i = 0; i < total; i += most) add_tile(first + i, std::min(most, total - i), from, end, page0);
     }
 
-    // Parts: about so many workgroups, none of less than so many blocks
-    constexpr int kPageFill = 768, kPageLeast = 8;
-    constexpr int kWideFill = 256, kWideLeast = 16;
-    long long blocks[2] = {0, 0};
-    for (const Tile &x : tiles) blocks[x.form > 1] += ceil_div(x.slot1 - x.slot0, kPageBlock);
-    const int parts[2] = {(int)std::max<long long>(kPageLeast, (blocks[0] * kv_heads + kPageFill - 1) / kPageFill),
-                          (int)std::max<long long>(kWideLeast, (blocks[1] * kv_heads + kWideFill - 1) / kWideFill)};
-    std::vector<int> count(n, 0);
-    std::vector<std::pair<int, int>> at;  // form and index of every item
+    // Long tiles are cut, in whole steps of the workgroup's waves.
+    p.wide = false;
+    long long blocks = 0;
+    int longest[2] = {1, 1};  // of the forms that the memory bounds, of the largest
     for (const Tile &x : tiles) {
-        const int nb = ceil_div(x.slot1 - x.slot0, kPageBlock), cuts = ceil_div(nb, parts[x.form > 1]);
-        const int each = ceil_div(nb, cuts);
+        const int nb = ceil_div(x.slot1 - x.slot0, kPageBlock);
+        p.wide = p.wide || x.form > 0;
+        blocks += nb;
+        longest[x.form > 1] = std::max(longest[x.form > 1], nb);
+    }
+    const float *cost = forms.wide_cost;
+    const int step = p.wide ? forms.wide_step : 4, least = 8;  // blocks of a step, of a part
+    auto whole = [&](long long x) { return (int)((std::max<long long>(x, least) + step - 1) / step * step); };
+    int part[2] = {longest[0], longest[1]};
+    if (!p.wide) {
+        // The memory bounds all of them, and a few workgroups a CU keep it busy.
+        part[0] = whole((blocks * kv_heads + forms.fill - 1) / forms.fill);
+    } else {
+        // Of a few lengths of the parts, those whose workgroups, handed out longest first, are done earliest.
+        const int machines = std::max(1, forms.wide_slots / kv_heads);
+        // joining: a launch and its traffic, in blocks (0.7 us for 16 KB a CU)
+        const double even = (double)blocks / machines, join = 6, unit = 8.0 * kv_heads * group * head_dim / 3.5e6;
+        static const double kOf[6] = {0, 1, 0.67, 0.5, 0.34, 0.25};
+        double best = 0;
+        std::vector<std::pair<float, int>> jobs;  // (time, how many)
+        std::vector<float> heap;
+        for (int i = 0; i < 6; i++)
+            for (int j = 0; j < 6; j++) {
+                const int len[2] = {i ? whole((long long)(even * kOf[i])) : longest[0], j ? whole((long long)(even * kOf[j])) : longest[1]};
+                if ((i && len[0] >= longest[0]) || (j && len[1] >= longest[1])) continue;
+                jobs.clear();
+                double units = 0;
+                for (const Tile &x : tiles) {
+                    const int nb = ceil_div(x.slot1 - x.slot0, kPageBlock), cuts = ceil_div(nb, len[x.form > 1]);
+                    jobs.push_back({ceil_div(nb, cuts) * cost[x.form] + forms.fixed, cuts});
+                    if (cuts > 1) units += (double)cuts * x.nq;
+                }
+                std::sort(jobs.begin(), jobs.end(), std::greater<>());
+                heap.assign(machines, 0.0f);  // a min-heap of when each machine is free
+                for (auto &w : jobs)
+                    for (int k = 0; k < w.second; k++) {
+                        std::pop_heap(heap.begin(), heap.end(), std::greater<>());
+                        heap.back() += w.first;
+                        std::push_heap(heap.begin(), heap.end(), std::greater<>());
+                    }
+                const double time = *std::max_element(heap.begin(), heap.end()) + (units > 0 ? join + units * unit : 0);
+                if ((i || j) && time >= best) continue;
+                best = time;
+                part[0] = len[0];
+                part[1] = len[1];
+            }
+    }
+    std::vector<int> count(n, 0);
+    for (const Tile &x : tiles) {
+        const int nb = ceil_div(x.slot1 - x.slot0, kPageBlock), cuts = ceil_div(nb, part[x.form > 1]);
+        const int each = (ceil_div(nb, cuts) + step - 1) / step * step;
         for (int b = 0; b < nb; b += each) {
             PageItem it{};
             it.q0 = x.q0;
             it.slot0 = x.slot0 + b * kPageBlock;
             it.slot1 = std::min(x.slot1, it.slot0 + each * kPageBlock);
             it.page0 = x.page0 + it.slot0 / P - x.slot0 / P;
+            it.form = x.form;
             while (it.nq < x.nq && p.order[x.q0 + it.nq].seen > it.slot0) it.nq++;
             it.smin = p.order[x.q0 + it.nq - 1].seen;
             for (int i = 0; i < it.nq; i++) count[p.order[x.q0 + i].query]++;
-            at.push_back({x.form, (int)p.items[x.form].size()});
-            p.items[x.form].push_back(it);
+            p.items.push_back(it);
         }
     }
+    std::stable_sort(p.items.begin(), p.items.end(), [&](const PageItem &a, const PageItem &b) {
+        return (a.slot1 - a.slot0) * cost[a.form] > (b.slot1 - b.slot0) * cost[b.form];
+    });
     std::vector<int> first(n + 1, 0);
     std::vector<char> joined(n, 0);
-    for (auto &a : at) {
-        PageItem &it = p.items[a.first][a.second];
+    for (PageItem &it : p.items) {
         bool alone = true;
         for (int i = 0; i < it.nq; i++) alone = alone && count[p.order[it.q0 + i].query] == 1;
         it.unit = alone ? -1 : p.num_units;
@@ -384,8 +448,7 @@ int page_plan(PageTable &t, const int32_t *s, const int32_t *seen, int n, int gr
     for (int i = 0; i < n; i++)
         if (joined[i] || !count[i]) p.joins.push_back({i, first[i], joined[i] ? count[i] : 0, 0});
     std::vector<int> next(first.begin(), first.end() - 1);
-    for (auto &a : at) {
-        const PageItem &it = p.items[a.first][a.second];
+    for (const PageItem &it : p.items) {
         if (it.unit < 0) continue;
         for (int i = 0; i < it.nq; i++) p.units[next[p.order[it.q0 + i].query]++] = it.unit + i;
     }

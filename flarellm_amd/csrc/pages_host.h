@@ -63,7 +63,7 @@ struct PageItem {
     int q0, nq, slot0, slot1, page0;
     int unit;  // partial result of the first query; -1: the item is all that its queries see
     int smin;  // fewest tokens that one of the queries sees
-    int pad;
+    int form;  // by its rows (query x head of a kv head), see PageForms
 };
 
 // A query in an item's order: its number, and how many tokens it sees.
@@ -77,11 +77,21 @@ struct PageJoin {
     int query, first, count, pad;
 };
 
-// Item forms, by rows (query x head of a kv head): one and two tiles of 16, 2 and 4 of 32.
-constexpr int kPageForms = 4, kPageRows[kPageForms] = {16, 32, 64, 128};
+// The forms of items that a cache's kernels have, and what the cuts of long items go by.
+// A launch without an item of a form above 0 has workgroups of 4 waves, about `fill` of
+// them; another has workgroups that take `wide_step` blocks at a time, `wide_slots` at
+// once on the chip, each for `fixed` and wide_cost a 32-token block, in units of a block
+// of the first form.
+struct PageForms {
+    int n, rows[3];
+    int fill;
+    float wide_cost[3], fixed;
+    int wide_step, wide_slots;
+};
 
 struct PagePlan {
-    std::vector<PageItem> items[kPageForms];
+    std::vector<PageItem> items;  // longest first
+    bool wide = false;            // an item of a form above 0
     std::vector<PageQuery> order;
     std::vector<int> page_ids, units;
     std::vector<PageJoin> joins;
@@ -89,8 +99,8 @@ struct PagePlan {
 };
 
 // seen[i] tokens of sequence s[i] for query i (checked against the table).
-// group: query heads per kv head; forms: how many of the item forms there are.  0, or a
-// code and table.error.
-int page_plan(PageTable &t, const int32_t *s, const int32_t *seen, int n, int group, int kv_heads, int forms, PagePlan &p);
+// group: query heads per kv head.  0, or a code and table.error.
+int page_plan(PageTable &t, const int32_t *s, const int32_t *seen, int n, int group, int kv_heads, int head_dim,
+              const PageForms &forms, PagePlan &p);
 
 }  // namespace fl

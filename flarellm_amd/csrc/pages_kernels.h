@@ -412,31 +412,26 @@ __device__ __forceinline__ void pg_join_row(const PageAttnArgs &a, const PageIte
     if (odd != 0.0f) *bad = 1;  // 0 * Inf and 0 * NaN are NaN
 }
 
-// One item (PageItem) and kv head per workgroup of 4 waves; wave w takes the item's
-// 32-slot blocks w, w + 4, ..  Each keeps (max, sum, O) of its blocks for NT x 16
-// rows (query x head), joined through LDS at the end.  K of a wave's next block is
-// loaded when the scores have been formed, V when O has been: half a block ahead.
+// Items of up to 16 NT rows (query x head): NW waves, wave w takes the item's 32-slot
+// blocks w, w + NW, ..  Each keeps (max, sum, O) of its blocks for NT x 16 rows, joined
+// through LDS at the end ([NW][16][D + 4] floats: O, max, sum of one tile).  K of a wave's
+// next block is loaded when the scores have been formed, V when O has been: half a
+// block ahead.  Bound by the memory: a block is 16 NT products for 16 KB (D = 128, binary16).
 //
 // Values that are not finite: slots behind the item's last token are taken out of V;
 // a token that some of the item's queries see and others do not has p = 0 for the
 // latter, and 0 * Inf is NaN, as is an Inf against a zero low part.  Every such case
 // leaves a NaN or Inf in O: such a row is then formed again, key by key.
-template <int FMT, int D, int NT>
-__global__ __launch_bounds__(256) void k_pages_attn(PageAttnArgs a) {
+template <int FMT, int D, int NT, int NW>
+__device__ __forceinline__ void pg_narrow(const PageAttnArgs &a, const PageItem &it, int kvh, float *lds, int *bad) {
     using Block = PgBlock<FMT, D>;
-    constexpr int QP = Block::QP, DT = D / 16;
-    // [4 waves][16 rows][D + 4]: O, max, sum (of one 16-row tile at a time)
-    constexpr int LROW = D + 4;
-    __shared__ __align__(16) float lds[4 * 16 * LROW];
-    __shared__ int bad_rows;
+    constexpr int QP = Block::QP, DT = D / 16, LROW = D + 4;
     const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int nkv = a.pool.nkv, kvh = blockIdx.x % nkv, G = a.group, nh = nkv * G;
-    const PageItem it = a.items[blockIdx.x / nkv];
+    const int nkv = a.pool.nkv, G = a.group;
     const int rows = it.nq * G, P = a.pool.P;
     const int nb = (it.slot1 - it.slot0 + 31) >> 5;
     const size_t layer_pages = (size_t)a.layer * a.pool.pages;
-    if (threadIdx.x == 0) bad_rows = 0;
 
     // block b: its (page, kv head), and its first slot in the page
     auto locate = [&](int b, size_t &head, int &slot) {
@@ -454,7 +449,7 @@ __global__ __launch_bounds__(256) void k_pages_attn(PageAttnArgs a) {
     blk.load_k(a.pool, head, slot, m, g);
     blk.load_v(a.pool, head, slot, m, g);
 
-    pg_stage_q<D, LROW, 256>(a, it, kvh, lds);
+    pg_stage_q<D, LROW, 64 * NW>(a, it, kvh, lds);
     __syncthreads();
     pu4_t q[NT][QP];
     float c[NT];
@@ -486,14 +481,14 @@ __global__ __launch_bounds__(256) void k_pages_attn(PageAttnArgs a) {
         for (int d = 0; d < DT; d++) o[n][d] = pf4_t{0, 0, 0, 0};
     }
 
-    for (int b = wave; b < nb; b += 4) {
+    for (int b = wave; b < nb; b += NW) {
         const int tok = it.slot0 + 32 * b;  // first token of the block
         pf4_t s[NT][2];
 #pragma unroll
         for (int n = 0; n < NT; n++) blk.scores(q[n], g, s[n]);
         size_t head2;
         int slot2;
-        locate(min(b + 4, last), head2, slot2);  // past the end: loaded, not used
+        locate(min(b + NW, last), head2, slot2);  // past the end: loaded, not used
         blk.load_k(a.pool, head2, slot2, m, g);
         if (tok + 32 > it.smin) {  // some query does not see every token
 #pragma unroll
@@ -532,8 +527,7 @@ __global__ __launch_bounds__(256) void k_pages_attn(PageAttnArgs a) {
         blk.load_v(a.pool, head2, slot2, m, g);
     }
 
-    // join the waves, one 16-row tile at a time: thread t has row t / 16 and the
-    // channels of t % 16
+    // join the waves, one 16-row tile at a time
 #pragma unroll
     for (int n = 0; n < NT; n++) {
         if (16 * n >= rows) break;
@@ -547,38 +541,29 @@ __global__ __launch_bounds__(256) void k_pages_attn(PageAttnArgs a) {
             w[D + 1] = l;
         }
         __syncthreads();
-        for (int r = threadIdx.x / (D / 4); r < min(16, rows - 16 * n); r += 256 / (D / 4))
-            pg_join_row<D, 4>(a, it, kvh, 16 * n + r, threadIdx.x % (D / 4) * 4, lds + r * LROW, 16 * LROW, &bad_rows);
+        for (int r = threadIdx.x / (D / 4); r < min(16, rows - 16 * n); r += 64 * NW / (D / 4))
+            pg_join_row<D, NW>(a, it, kvh, 16 * n + r, threadIdx.x % (D / 4) * 4, lds + r * LROW, 16 * LROW, bad);
     }
-    __syncthreads();
-    if (bad_rows) pg_rows_again<FMT, D>(a, it, kvh, lds);
 }
 
-// Items of up to 32 R rows: R row groups of 32 x 8 / R key lanes in 8 waves (R = 2, 4), or
-// one x 4 in 4 (R = 1).  A step is 128 tokens, K and V of its four 32-slot blocks copied
-// memory -> LDS one step ahead (of 8 waves, each copies K or V of one block, of 4 each
-// both of its own, and never waits for the others); a key lane takes one of them or two.  Products are
+// Items of up to 32 R rows, binary16: 8 waves, R row groups of 32 x 8 / R key lanes.  A step
+// is 128 tokens, K and V of its four 32-slot blocks copied memory -> LDS one step ahead
+// (wave w copies K or V of one block); a key lane takes R / 2 of them.  Products are
 // 32 x 32 x 16: a query row is a lane (mod 32), the K rows enter with index bits 2 and 3
 // swapped so that scores i = 8 mm + j of a lane are slots 16 mm + 8 (lane / 32) + j, the
-// operand of O^T = V^T P^T.  Bound by the matrix issue: 64 products of 32 cycles per block
-// and row group, two waves a SIMD, whose softmax runs beside the other's products.
+// operand of O^T = V^T P^T.  smem: two steps of K and V; at the end [8][32][D + 4] floats.
 template <int D, int R>
-__global__ __launch_bounds__(R == 1 ? 256 : 512) __attribute__((amdgpu_waves_per_eu(R == 1 ? 1 : 2, 2))) void k_pages_wide(
-    PageAttnArgs a) {
-    constexpr int FMT = FL_KV_F16, NW = R == 1 ? 4 : 8, KL = NW / R, NB = 4 / KL;
+__device__ __forceinline__ void pg_wide(const PageAttnArgs &a, const PageItem &it, int kvh, char *smem, int *bad) {
+    constexpr int FMT = FL_KV_F16, KL = 8 / R, NB = 4 / KL;
     constexpr int KS = D / 16, DT = D / 32, CH = D / 8, BLK = 32 * D * 2;  // BLK: bytes of a block's K (or V)
     constexpr int LROW = D + 4;
-    extern __shared__ __align__(16) char smem[];  // 2 x (4 K blocks, 4 V blocks); at the end [waves][32][LROW]
-    __shared__ int bad_rows;
     const int lane = threadIdx.x & 63, l31 = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), rg = wave % R, kl = wave / R;
-    const int nkv = a.pool.nkv, kvh = blockIdx.x % nkv, G = a.group;
-    const PageItem it = a.items[blockIdx.x / nkv];
+    const int nkv = a.pool.nkv, G = a.group;
     const int rows = it.nq * G, P = a.pool.P;
     const int nb = (it.slot1 - it.slot0 + 31) >> 5, nit = (nb + 3) >> 2;
     const size_t layer_pages = (size_t)a.layer * a.pool.pages;
     const bool live = 32 * rg < rows;  // wave-uniform
-    if (threadIdx.x == 0) bad_rows = 0;
 
     // chunk p (16 B) of a K block in LDS holds chunk c ^ g(row) of its row, g from row bits
     // 0, 1, 3 (the rows that 8 lanes read together differ in those); of a V block, chunk
@@ -590,23 +575,22 @@ __global__ __launch_bounds__(R == 1 ? 256 : 512) __attribute__((amdgpu_waves_per
         const int w = wave & 3, b = min(4 * step + w, nb - 1), tok = it.slot0 + 32 * b;
         const int page = __builtin_amdgcn_readfirstlane(a.page_ids[it.page0 + tok / P - it.slot0 / P]);
         const size_t at = (((layer_pages + page) * nkv + kvh) * P + tok % P) * D * 2;
-        char *dst = smem + (size_t)(8 * buf + w) * BLK;
-        if (R == 1 || wave < 4) {
+        char *dst = smem + (size_t)(8 * buf + wave) * BLK;
+        if (wave < 4) {
 #pragma unroll
             for (int u = 0; u < BLK / 1024; u++)
                 copy_to_lds((const char *)a.pool.k + at + u * 1024 + (((u * 64 / CH) & 8) ? kplace ^ 64 : kplace), dst + u * 1024);
-        }
-        if (R == 1 || wave >= 4) {
+        } else {
 #pragma unroll
             for (int u = 0; u < BLK / 1024; u++)
-                copy_to_lds((const char *)a.pool.v + at + u * 1024 + vplace, dst + 4 * BLK + u * 1024);
+                copy_to_lds((const char *)a.pool.v + at + u * 1024 + vplace, dst + u * 1024);
         }
     };
     copy(0, 0);
 
     // the queries, in the second buffer until its first copy
     float *lds = (float *)smem, *ql = (float *)(smem + 8 * BLK);
-    pg_stage_q<D, LROW, 64 * NW>(a, it, kvh, ql);
+    pg_stage_q<D, LROW, 512>(a, it, kvh, ql);
     __syncthreads();
     const int r0 = min(32 * rg + l31, rows - 1);
     const int seen = a.order[it.q0 + r0 / G].seen;
@@ -625,7 +609,6 @@ __global__ __launch_bounds__(R == 1 ? 256 : 512) __attribute__((amdgpu_waves_per
         for (int j = 0; j < 8; j++) x[j] = qp[16 * k + j] * mul;
         pg_split(x, q[k][0], q[k][1]);
     }
-    if (R == 1) __syncthreads();  // (other waves' copies into the second buffer)
     const pf16_t zero = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
     pf16_t o[DT];
 #pragma unroll
@@ -642,22 +625,19 @@ __global__ __launch_bounds__(R == 1 ? 256 : 512) __attribute__((amdgpu_waves_per
 
     for (int step = 0; step < nit; step++) {
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-        if (R > 1) __builtin_amdgcn_s_barrier();  // this step has landed, and nobody reads the other buffer
+        __builtin_amdgcn_s_barrier();  // this step has landed, and nobody reads the other buffer
         asm volatile("" ::: "memory");
         const int buf = step & 1;
         if (step + 1 < nit) {
             copy(step + 1, buf ^ 1);
         } else if (const int over = (it.slot1 - it.slot0) & 31; over) {
             // slots behind the item's last token: whatever is there must not meet a zero
-            const int lastb = (nb - 1) & 3;
-            char *vb = smem + (size_t)(8 * buf + 4 + lastb) * BLK;
-            if (R > 1 || wave == lastb)
-                for (int i = R > 1 ? threadIdx.x : lane; i < 32 * D; i += R > 1 ? 512 : 64) {
-                    const int d = i >> 5, s = i & 31;
-                    if (s >= over) *(uint16_t *)(vb + d * 64 + (((s >> 3) ^ ((d >> 1) & 3)) * 16) + (s & 7) * 2) = 0;
-                }
-            if (R > 1) __syncthreads();
-            else asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            char *vb = smem + (size_t)(8 * buf + 4 + ((nb - 1) & 3)) * BLK;
+            for (int i = threadIdx.x; i < 32 * D; i += 512) {
+                const int d = i >> 5, s = i & 31;
+                if (s >= over) *(uint16_t *)(vb + d * 64 + (((s >> 3) ^ ((d >> 1) & 3)) * 16) + (s & 7) * 2) = 0;
+            }
+            __syncthreads();
         }
         if (!live) continue;
         // Operands are read from LDS a phase ahead: V before the softmax, the next
@@ -744,10 +724,42 @@ __global__ __launch_bounds__(R == 1 ? 256 : 512) __attribute__((amdgpu_waves_per
         }
     }
     __syncthreads();
-    for (int r = threadIdx.x / (D / 4); r < rows; r += 64 * NW / (D / 4))
-        pg_join_row<D, KL>(a, it, kvh, r, threadIdx.x % (D / 4) * 4, lds + (size_t)r * LROW, 32 * R * LROW, &bad_rows);
+    for (int r = threadIdx.x / (D / 4); r < rows; r += 512 / (D / 4))
+        pg_join_row<D, KL>(a, it, kvh, r, threadIdx.x % (D / 4) * 4, lds + (size_t)r * LROW, 32 * R * LROW, bad);
+}
+
+// One item (PageItem) and kv head per workgroup; the kv head is the faster index, so that
+// with 8 of them the items of a head share an XCD's L2.
+
+// Items of up to 16 rows (FORMS = 1), or up to 32: 4 waves.
+template <int FMT, int D, int FORMS>
+__global__ __launch_bounds__(256) void k_pages_attn(PageAttnArgs a) {
+    __shared__ __align__(16) float lds[4 * 16 * (D + 4)];
+    __shared__ int bad;
+    const int kvh = blockIdx.x % a.pool.nkv;
+    const PageItem it = a.items[blockIdx.x / a.pool.nkv];
+    if (threadIdx.x == 0) bad = 0;
+    if (FORMS == 1 || it.form == 0) pg_narrow<FMT, D, 1, 4>(a, it, kvh, lds, &bad);
+    else pg_narrow<FMT, D, FORMS, 4>(a, it, kvh, lds, &bad);
     __syncthreads();
-    if (bad_rows) pg_rows_again<FMT, D>(a, it, kvh, lds);
+    if (bad) pg_rows_again<FMT, D>(a, it, kvh, lds);
+}
+
+// binary16, items of up to 128 rows: 8 waves, one workgroup a CU.  (In one launch, so that
+// items of many rows, which the matrix cores bound, run beside those of few, which the
+// memory does.)
+template <int D>
+__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) void k_pages_attn_wide(PageAttnArgs a) {
+    extern __shared__ __align__(16) char smem[];
+    __shared__ int bad;
+    const int kvh = blockIdx.x % a.pool.nkv;
+    const PageItem it = a.items[blockIdx.x / a.pool.nkv];
+    if (threadIdx.x == 0) bad = 0;
+    if (it.form == 0) pg_narrow<FL_KV_F16, D, 1, 8>(a, it, kvh, (float *)smem, &bad);
+    else if (it.form == 1) pg_wide<D, 2>(a, it, kvh, smem, &bad);
+    else pg_wide<D, 4>(a, it, kvh, smem, &bad);
+    __syncthreads();
+    if (bad) pg_rows_again<FL_KV_F16, D>(a, it, kvh, (float *)smem);
 }
 
 // Partial results of a query joined: a workgroup takes 128 channels, 4 a thread, and

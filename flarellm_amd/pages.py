@@ -64,6 +64,7 @@ class PagedKv:
         self.stream = torch.cuda.ExternalStream(backend.stream, device=self.device)
         self._stream = self.stream.cuda_stream
         self._row = (kv_heads, head_dim)
+        self._before, self._behind = torch.cuda.Event(), torch.cuda.Event()  # (kept: making one costs 10 us)
         # the memory may be what earlier work of the current stream still uses
         self.stream.wait_stream(torch.cuda.current_stream(self.device))
         h = C.c_void_p()
@@ -99,11 +100,13 @@ class PagedKv:
         if current == self._stream:
             return self._call(fn, *args)
         current = torch.cuda.current_stream(self.device)
-        self.stream.wait_stream(current)
+        self._before.record(current)
+        self.stream.wait_event(self._before)
         try:
             self._call(fn, *args)
         finally:
-            current.wait_stream(self.stream)
+            self._behind.record(self.stream)
+            current.wait_event(self._behind)
 
     def _rows(self, t, what: str, shape):
         """A float32 tensor on this device whose last dimensions are `shape`, without gaps between them."""
