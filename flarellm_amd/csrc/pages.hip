@@ -261,8 +261,8 @@ struct LaunchRead {
 // Costs fitted to measured calls (a block of 32 tokens of D = 128: 0.7 us where the memory
 // bounds it, 1.1 for 128 rows).
 const PageForms &forms_of(const fl_pages *p) {
-    static const PageForms f16 = {3, {16, 64, 128}, 768, {1, 1, 1.6f}, 6, 8, 256};
-    static const PageForms other = {2, {16, 32, 0}, 768, {2, 3, 0}, 6, 4, 512};
+    static const PageForms f16 = {3, {16, 64, 128}, 512, {1, 1, 1.6f}, 6, 8, 256};
+    static const PageForms other = {2, {16, 32, 0}, 512, {2, 3, 0}, 6, 4, 512};
     return p->cfg.kv_format == FL_KV_F16 ? f16 : other;
 }
 
@@ -342,7 +342,9 @@ int fl_pages_create(fl_ctx *ctx, const fl_pages_config *cfg, void *k, void *v, v
     p->ctx = ctx;
     p->cfg = *cfg;
     p->pool = PagePool{k, v, (uint16_t *)k_scale, (uint16_t *)v_scale, cfg->num_layers, cfg->num_pages, cfg->page_size,
-                       cfg->num_kv_heads};
+                       cfg->num_kv_heads, cfg->page_size / kPageBlock, 0};
+    // exact for x < 2^19 blocks: the error x / 2^32 is below 1 / per (per <= 128; per = 1 has no 32-bit inverse)
+    p->pool.per_inv = p->pool.per > 1 ? (uint32_t)(((1ull << 32) + p->pool.per - 1) / p->pool.per) : 0;
     if (ctx) {
         p->device = fl_ctx_device(ctx);
         p->stream = (hipStream_t)fl_ctx_stream(ctx);

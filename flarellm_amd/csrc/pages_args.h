@@ -14,6 +14,8 @@ struct PagePool {
     void *k, *v;
     uint16_t *ks, *vs;  // Q8
     int layers, pages, P, nkv;
+    int per;               // blocks (32 slots) of a page
+    uint32_t per_inv;      // floor(x / per) = x * per_inv >> 32 for blocks x of a sequence
 };
 
 struct PageAttnArgs {

@@ -377,7 +377,15 @@ int page_plan(PageTable &t, const int32_t *s, const int32_t *seen, int n, int gr
     int part[2] = {longest[0], longest[1]};
     if (!p.wide) {
         // The memory bounds all of them, and a few workgroups a CU keep it busy.
-        part[0] = whole((blocks * kv_heads + forms.fill - 1) / forms.fill);
+        // As many as it takes at once where that does for all, or else twice as many: 32768
+        // tokens alone 28.6 us in 512 workgroups and 35.9 in 1024, 16 sequences of 40 to 7800
+        // tokens 46.8 and 43.6.
+        for (int f = 1; f <= 2; f++) {
+            part[0] = whole((blocks * kv_heads + f * forms.fill - 1) / (f * forms.fill));
+            long long n = 0;
+            for (const Tile &x : tiles) n += ceil_div(ceil_div(x.slot1 - x.slot0, kPageBlock), part[0]);
+            if (n * kv_heads <= forms.fill) break;
+        }
     } else {
         // Of a few lengths of the parts, those whose workgroups, handed out longest first, are done earliest.
         const int machines = std::max(1, forms.wide_slots / kv_heads);

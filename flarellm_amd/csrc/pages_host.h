@@ -78,8 +78,8 @@ struct PageJoin {
 };
 
 // The forms of items that a cache's kernels have, and what the cuts of long items go by.
-// A launch without an item of a form above 0 has workgroups of 4 waves, about `fill` of
-// them; another has workgroups that take `wide_step` blocks at a time, `wide_slots` at
+// A launch without an item of a form above 0 has workgroups of 4 waves, `fill` of them at
+// once on the chip; another has workgroups that take `wide_step` blocks at a time, `wide_slots` at
 // once on the chip, each for `fixed` and wide_cost a 32-token block, in units of a block
 // of the first form.
 struct PageForms {

@@ -304,6 +304,29 @@ struct PgBlock<FL_KV_F32, D> {
     }
 };
 
+// Where an item's blocks are.  Its page numbers go through the scalar cache, asked for a
+// block (or step) ahead: as vector loads they would wait behind the keys' and values'.
+struct PgWalk {
+    const __attribute__((address_space(4))) int *ids;
+    int blk0, first, per;
+    uint32_t inv;
+    __device__ __forceinline__ int page_of(int blk) const { return inv ? (int)(((uint64_t)(uint32_t)blk * inv) >> 32) : blk; }
+    __device__ __forceinline__ PgWalk(const PageAttnArgs &a, const PageItem &it)
+        : ids((const __attribute__((address_space(4))) int *)(a.page_ids + it.page0)), blk0(it.slot0 >> 5), per(a.pool.per),
+          inv(a.pool.per_inv) {
+        first = page_of(blk0);
+    }
+    __device__ __forceinline__ int page(int b) const { return ids[page_of(blk0 + b) - first]; }
+    // first slot of block b in its page
+    __device__ __forceinline__ int slot(int b) const { return 32 * (blk0 + b - page_of(blk0 + b) * per); }
+};
+// An item, through the scalar cache
+__device__ __forceinline__ PageItem pg_item(const PageAttnArgs &a, int i) {
+    typedef int i8_t __attribute__((ext_vector_type(8)));
+    const i8_t w = ((const __attribute__((address_space(4))) i8_t *)a.items)[i];
+    return PageItem{w[0], w[1], w[2], w[3], w[4], w[5], w[6], w[7]};
+}
+
 // An item's rows key by key, where some value was not finite: 2^kShift times the
 // sum and O, in base 2 relative to the largest score, as the tiles have them (all rows
 // of the item; this is rare).  lds: 260 floats.
@@ -433,21 +456,16 @@ __device__ __forceinline__ void pg_narrow(const PageAttnArgs &a, const PageItem 
     const int nb = (it.slot1 - it.slot0 + 31) >> 5;
     const size_t layer_pages = (size_t)a.layer * a.pool.pages;
 
-    // block b: its (page, kv head), and its first slot in the page
-    auto locate = [&](int b, size_t &head, int &slot) {
-        const int tok = it.slot0 + 32 * b, first = it.slot0 / P;
-        const int page = __builtin_amdgcn_readfirstlane(a.page_ids[it.page0 + tok / P - first]);
-        slot = tok % P;
-        head = (layer_pages + page) * nkv + kvh;
-    };
-
+    const PgWalk walk(a, it);
+    const int last = nb - 1;
     Block blk;
-    size_t head;
-    int slot;
-    const int last = max(0, nb - 1);
-    locate(min(wave, last), head, slot);
-    blk.load_k(a.pool, head, slot, m, g);
-    blk.load_v(a.pool, head, slot, m, g);
+    int b0 = min(wave, last), b1 = min(wave + NW, last);  // this block and the next: past the end, the last one
+    int page = walk.page(b1);
+    {
+        const size_t head = (layer_pages + walk.page(b0)) * nkv + kvh;
+        blk.load_k(a.pool, head, walk.slot(b0), m, g);
+        blk.load_v(a.pool, head, walk.slot(b0), m, g);
+    }
 
     pg_stage_q<D, LROW, 64 * NW>(a, it, kvh, lds);
     __syncthreads();
@@ -486,10 +504,11 @@ __device__ __forceinline__ void pg_narrow(const PageAttnArgs &a, const PageItem 
         pf4_t s[NT][2];
 #pragma unroll
         for (int n = 0; n < NT; n++) blk.scores(q[n], g, s[n]);
-        size_t head2;
-        int slot2;
-        locate(min(b + NW, last), head2, slot2);  // past the end: loaded, not used
-        blk.load_k(a.pool, head2, slot2, m, g);
+        const size_t head = (layer_pages + page) * nkv + kvh;
+        const int slot = walk.slot(b1);
+        blk.load_k(a.pool, head, slot, m, g);
+        b1 = min(b1 + NW, last);
+        page = walk.page(b1);
         if (tok + 32 > it.smin) {  // some query does not see every token
 #pragma unroll
             for (int n = 0; n < NT; n++)
@@ -524,7 +543,7 @@ __device__ __forceinline__ void pg_narrow(const PageAttnArgs &a, const PageItem 
             }
             blk.add_pv(p, g, o[n]);
         }
-        blk.load_v(a.pool, head2, slot2, m, g);
+        blk.load_v(a.pool, head, slot, m, g);
     }
 
     // join the waves, one 16-row tile at a time
@@ -571,10 +590,12 @@ __device__ __forceinline__ void pg_wide(const PageAttnArgs &a, const PageItem &i
     // them, but for row bit 3, which is a bit of the copy's number.
     const int r8 = lane / CH;
     const int kplace = 16 * (r8 * CH + ((lane % CH) ^ (r8 & 3))), vplace = 16 * ((lane & ~3) | ((lane & 3) ^ ((lane >> 3) & 3)));
+    const PgWalk walk(a, it);
+    int page = walk.page(min(wave & 3, nb - 1));
     auto copy = [&](int step, int buf) {
-        const int w = wave & 3, b = min(4 * step + w, nb - 1), tok = it.slot0 + 32 * b;
-        const int page = __builtin_amdgcn_readfirstlane(a.page_ids[it.page0 + tok / P - it.slot0 / P]);
-        const size_t at = (((layer_pages + page) * nkv + kvh) * P + tok % P) * D * 2;
+        const int b = min(4 * step + (wave & 3), nb - 1);
+        const size_t at = (((layer_pages + page) * nkv + kvh) * P + walk.slot(b)) * D * 2;
+        page = walk.page(min(b + 4, nb - 1));  // the next step's
         char *dst = smem + (size_t)(8 * buf + wave) * BLK;
         if (wave < 4) {
 #pragma unroll
@@ -737,7 +758,7 @@ __global__ __launch_bounds__(256) void k_pages_attn(PageAttnArgs a) {
     __shared__ __align__(16) float lds[4 * 16 * (D + 4)];
     __shared__ int bad;
     const int kvh = blockIdx.x % a.pool.nkv;
-    const PageItem it = a.items[blockIdx.x / a.pool.nkv];
+    const PageItem it = pg_item(a, blockIdx.x / a.pool.nkv);
     if (threadIdx.x == 0) bad = 0;
     if (FORMS == 1 || it.form == 0) pg_narrow<FMT, D, 1, 4>(a, it, kvh, lds, &bad);
     else pg_narrow<FMT, D, FORMS, 4>(a, it, kvh, lds, &bad);
@@ -753,7 +774,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     extern __shared__ __align__(16) char smem[];
     __shared__ int bad;
     const int kvh = blockIdx.x % a.pool.nkv;
-    const PageItem it = a.items[blockIdx.x / a.pool.nkv];
+    const PageItem it = pg_item(a, blockIdx.x / a.pool.nkv);
     if (threadIdx.x == 0) bad = 0;
     if (it.form == 0) pg_narrow<FL_KV_F16, D, 1, 8>(a, it, kvh, (float *)smem, &bad);
     else if (it.form == 1) pg_wide<D, 2>(a, it, kvh, smem, &bad);
