@@ -45,7 +45,7 @@ struct fl_pages {
     int plan_heads = 0;
     uint64_t plan_version = 0;
     size_t plan_order = 0, plan_pages = 0, plan_units = 0, plan_joins = 0;  // offsets
-    DevBuf d_plan, d_slots, d_read, d_copies, ws;
+    DevBuf d_plan, d_runs, d_read, d_copies, ws;
     Stage stages[kStages];
     int stage = 0;
 };
@@ -238,11 +238,11 @@ struct LaunchAttn {
 struct LaunchWrite {
     hipStream_t st;
     const PageWriteArgs &a;
-    const PageSlots &slots;
+    const PageRuns &runs;
+    int n, layers;
     template <int FMT, int D>
     int operator()() const {
-        const long long total = (long long)a.layers * a.n * a.pool.nkv * (D / 32) * 2;
-        hipLaunchKernelGGL((k_pages_write<FMT, D>), dim3((unsigned)((total + 255) / 256)), dim3(256), 0, st, a, slots);
+        hipLaunchKernelGGL((k_pages_write<FMT, D>), dim3(n, a.pool.nkv, layers), dim3(256), 0, st, a, runs);
         return (int)hipGetLastError();
     }
 };
@@ -250,13 +250,23 @@ struct LaunchWrite {
 struct LaunchRead {
     hipStream_t st;
     const PageReadArgs &a;
+    const PageRuns &runs;
+    int n;
     template <int FMT, int D>
     int operator()() const {
-        const long long total = (long long)a.n * a.pool.nkv * D;
-        hipLaunchKernelGGL((k_pages_read<FMT, D>), dim3((unsigned)((total + 255) / 256)), dim3(256), 0, st, a);
+        hipLaunchKernelGGL((k_pages_read<FMT, D>), dim3(n, a.pool.nkv), dim3(256), 0, st, a, runs);
         return (int)hipGetLastError();
     }
 };
+
+// Runs as an argument of a launch; `dev` holds those of a long list already.
+PageRuns runs_of(const std::vector<PageRun> &v, const DevBuf &dev) {
+    PageRuns r;
+    r.list = nullptr;
+    if (v.size() > kInlineRuns) r.list = (const PageRun *)dev.p;
+    else memcpy(r.some, v.data(), v.size() * sizeof(PageRun));
+    return r;
+}
 
 // Costs fitted to measured calls (a block of 32 tokens of D = 128: 0.7 us where the memory
 // bounds it, 1.1 for 128 rows).
@@ -368,7 +378,7 @@ void fl_pages_destroy(fl_pages *p) {
     if (p->ctx) {
         OnDevice on(p);
         // (hipFree waits for the device, so the context may be gone already)
-        for (DevBuf *b : {&p->d_plan, &p->d_slots, &p->d_read, &p->d_copies, &p->ws})
+        for (DevBuf *b : {&p->d_plan, &p->d_runs, &p->d_read, &p->d_copies, &p->ws})
             if (b->p) (void)hipFree(b->p);
         for (Stage &s : p->stages) {
             if (s.done) (void)hipEventDestroy(s.done);
@@ -412,13 +422,14 @@ int fl_pages_extend(fl_pages *p, const int32_t *seqs, const int32_t *counts, int
     if (!p->ctx) return on_table(p, [&](PageTable &t) { return t.extend(seqs, counts, n); });
     PGTRY(check_stream(p));
     OnDevice on(p);
-    // room for the slots first: nothing fails behind the bookkeeping
-    long long tokens = 0;
-    for (int i = 0; i < n && counts; i++) tokens += std::min(std::max(counts[i], 0), p->cfg.max_seq_len);
-    tokens = std::min(tokens, (long long)p->cfg.num_pages * p->cfg.page_size);
-    if (tokens > kInlineSlots) PGTRY(ensure(p, p->d_slots, (size_t)tokens * sizeof(int)));
+    // room for the runs first: nothing fails behind the bookkeeping
+    long long most = 0;
+    for (int i = 0; i < n && counts; i++) most += std::min(std::max(counts[i], 0), p->cfg.max_seq_len) / kPageBlock + 2;
+    most = std::min(most, (long long)p->cfg.num_pages * p->pool.per + n);
+    if (most > kInlineRuns) PGTRY(ensure(p, p->d_runs, (size_t)most * sizeof(PageRun)));
     PGTRY(on_table(p, [&](PageTable &t) { return t.extend(seqs, counts, n); }));
-    if (p->t.slots.size() > kInlineSlots) PGTRY(upload(p, p->d_slots, p->t.slots.data(), p->t.slots.size() * sizeof(int)));
+    const auto &r = p->t.runs;
+    if (r.size() > kInlineRuns) PGTRY(upload(p, p->d_runs, r.data(), r.size() * sizeof(PageRun)));
     return run_copies(p);
 }
 
@@ -430,22 +441,19 @@ int fl_pages_write(fl_pages *p, int layer, int layers, const float *k, const flo
     if (!k || !v) return fail(p, FL_E_INVALID, "null keys or values");
     if (((uintptr_t)k | (uintptr_t)v) % 4) return fail(p, FL_E_INVALID, "keys or values are not aligned");
     if (row_stride < row) return fail(p, FL_E_INVALID, "rows of %zu values %zu apart", row, row_stride);
-    if (!p->t.slots_valid) return fail(p, FL_E_STATE, "fl_pages_write follows fl_pages_extend, with no other change between");
-    if (p->t.slots.empty()) return 0;
+    if (!p->t.runs_valid) return fail(p, FL_E_STATE, "fl_pages_write follows fl_pages_extend, with no other change between");
+    if (!p->t.tokens) return 0;
     OnDevice on(p);
     PageWriteArgs a{};
     a.pool = p->pool;
-    PageSlots slots;
-    slots.list = nullptr;
-    if (p->t.slots.size() > kInlineSlots) slots.list = (const int *)p->d_slots.p;
-    else memcpy(slots.some, p->t.slots.data(), p->t.slots.size() * sizeof(int));
     a.k = k;
     a.v = v;
     a.stride = (long long)row_stride;
     a.layer0 = layer;
-    a.layers = layers;
-    a.n = (int)p->t.slots.size();
-    PGCHK(p, (hipError_t)with_form(p->cfg.kv_format, p->cfg.head_dim, LaunchWrite{p->stream, a, slots}));
+    a.n = p->t.tokens;
+    const int n = (int)p->t.runs.size();
+    PGCHK(p, (hipError_t)with_form(p->cfg.kv_format, p->cfg.head_dim,
+                                   LaunchWrite{p->stream, a, runs_of(p->t.runs, p->d_runs), n, layers}));
     return 0;
 }
 
@@ -455,7 +463,7 @@ int fl_pages_read(fl_pages *p, int layer, const int32_t *seqs, const int32_t *st
     PGTRY(check_layers(p, layer, 1));
     PGTRY(check_stream(p));
     if (n < 0 || (n > 0 && (!seqs || !starts || !counts))) return fail(p, FL_E_INVALID, "bad sequence list");
-    std::vector<int> slots;
+    std::vector<PageRun> runs;
     PGTRY(on_table(p, [&](PageTable &t) {
         long long total = 0;
         for (int i = 0; i < n; i++) {
@@ -470,18 +478,20 @@ int fl_pages_read(fl_pages *p, int layer, const int32_t *seqs, const int32_t *st
             t.error = "too many tokens";
             return FL_E_INVALID;
         }
-        slots.reserve(total);
-        for (int i = 0; i < n; i++)
-            for (int j = starts[i]; j < starts[i] + counts[i]; j++)
-                slots.push_back(t.row(seqs[i])[j / t.page_size] * t.page_size + j % t.page_size);
+        int token = 0;
+        for (int i = 0; i < n; i++) {
+            t.add_runs(seqs[i], starts[i], starts[i] + counts[i], token, runs);
+            token += counts[i];
+        }
         return 0;
     }));
-    if (slots.empty()) return 0;
+    if (runs.empty()) return 0;
     if (!k && !v) return fail(p, FL_E_INVALID, "null keys and values");
     OnDevice on(p);
-    PGTRY(upload(p, p->d_read, slots.data(), slots.size() * sizeof(int)));
-    PageReadArgs a{p->pool, (const int *)p->d_read.p, k, v, layer, (int)slots.size()};
-    PGCHK(p, (hipError_t)with_form(p->cfg.kv_format, p->cfg.head_dim, LaunchRead{p->stream, a}));
+    if (runs.size() > kInlineRuns) PGTRY(upload(p, p->d_read, runs.data(), runs.size() * sizeof(PageRun)));
+    PageReadArgs a{p->pool, k, v, layer};
+    PGCHK(p, (hipError_t)with_form(p->cfg.kv_format, p->cfg.head_dim,
+                                   LaunchRead{p->stream, a, runs_of(runs, p->d_read), (int)runs.size()}));
     return 0;
 }
 
@@ -529,7 +539,7 @@ int fl_pages_attention(fl_pages *p, int layer, const float *q, size_t q_stride, 
 
 int fl_pages_len(const fl_pages *p, int seq) { return p && seq >= 0 && seq < p->t.seqs ? p->t.len[seq] : -1; }
 
-int fl_pages_pending(const fl_pages *p) { return p && p->t.slots_valid ? (int)p->t.slots.size() : -1; }
+int fl_pages_pending(const fl_pages *p) { return p && p->t.runs_valid ? p->t.tokens : -1; }
 
 int fl_pages_free_count(const fl_pages *p) { return p ? p->t.free_pages : -1; }
 

@@ -41,10 +41,10 @@ struct PageJoinArgs {
 
 // Short lists go with the launch (a copy to the device costs the host 5 us and the
 // stream 3); longer ones are in device memory.
-constexpr int kInlineSlots = 256, kInlineCopies = 96;
-struct PageSlots {
-    const int *list;       // page * P + slot of each token; nullptr: `some`
-    int some[kInlineSlots];
+constexpr int kInlineRuns = 128, kInlineCopies = 96;
+struct PageRuns {
+    const PageRun *list;   // nullptr: `some`
+    PageRun some[kInlineRuns];
 };
 struct PageCopies {
     const PageCopy *list;  // nullptr: `some`
@@ -55,14 +55,13 @@ struct PageWriteArgs {
     PagePool pool;
     const float *k, *v;    // token i, kv head h at (layer * n + i) * stride + h * D
     long long stride;
-    int layer0, layers, n;
+    int layer0, n;
 };
 
 struct PageReadArgs {
     PagePool pool;
-    const int *slots;
     float *k, *v;          // [n][nkv * D]
-    int layer, n;
+    int layer;
 };
 
 }  // namespace fl

@@ -74,6 +74,16 @@ int PageTable::blocks_of(int s, int i) const {
     return ceil_div(std::min(page_size, len[s] - i * page_size), kPageBlock);
 }
 
+void PageTable::add_runs(int s, int from, int to, int token, std::vector<PageRun> &out) const {
+    const int *r = row(s);
+    while (from < to) {
+        const int slot = from % kPageBlock, n = std::min(kPageBlock - slot, to - from);
+        out.push_back({(r[from / page_size] * page_size + from % page_size) / kPageBlock, token, (short)slot, (short)n});
+        from += n;
+        token += n;
+    }
+}
+
 int PageTable::fork(const int32_t *src, const int32_t *dst, const int32_t *lens, int n) {
     if (int rc = check_seqs(src, n, false)) return rc;
     if (int rc = check_seqs(dst, n, true)) return rc;
@@ -90,7 +100,7 @@ int PageTable::fork(const int32_t *src, const int32_t *dst, const int32_t *lens,
         std::copy(from, from + m, row(dst[i]));
         for (int j = 0; j < m; j++) ref[from[j]]++;
     }
-    slots_valid = false;
+    runs_valid = false;
     version++;
     return 0;
 }
@@ -115,7 +125,7 @@ int PageTable::copy(const int32_t *src, const int32_t *dst, int n) {
             copies.push_back({row(src[i])[j], g, blocks_of(src[i], j)});
         }
     }
-    slots_valid = false;
+    runs_valid = false;
     version++;
     return 0;
 }
@@ -131,7 +141,7 @@ int PageTable::release(const int32_t *s, int n) {
         }
         len[s[i]] = 0;
     }
-    slots_valid = false;
+    runs_valid = false;
     version++;
     return 0;
 }
@@ -152,7 +162,7 @@ int PageTable::truncate(const int32_t *s, const int32_t *lens, int n) {
             r[j] = -1;
         }
     }
-    slots_valid = false;
+    runs_valid = false;
     version++;
     return 0;
 }
@@ -184,13 +194,17 @@ int PageTable::extend(const int32_t *s, const int32_t *counts, int n) {
         i = j;
     }
     if (need > free_pages) return fail(FL_E_OOM, "%lld pages needed, %d free", need, free_pages);
-    std::vector<int> out;
-    out.reserve(tokens);
+    size_t most = 0;
+    for (int i = 0; i < n; i++) most += counts[i] / kPageBlock + 2;
+    std::vector<PageRun> out;
+    out.reserve(most);
     copies.clear();
     copies.reserve(left.size());
-    slots.swap(out);
+    runs.swap(out);
+    this->tokens = 0;
     for (int i = 0; i < n; i++) {
-        int *r = row(s[i]), at = len[s[i]];
+        int *r = row(s[i]);
+        const int at = len[s[i]];
         const int last = held(s[i]) - 1;
         if (counts[i] && at % page_size && ref[r[last]] > 1) {
             const int g = take();
@@ -200,9 +214,10 @@ int PageTable::extend(const int32_t *s, const int32_t *counts, int n) {
         }
         len[s[i]] += counts[i];
         for (int j = last + 1; j < held(s[i]); j++) r[j] = take();
-        for (; at < len[s[i]]; at++) slots.push_back(r[at / page_size] * page_size + at % page_size);
+        add_runs(s[i], at, len[s[i]], this->tokens, runs);
+        this->tokens += counts[i];
     }
-    slots_valid = true;
+    runs_valid = true;
     version++;
     return 0;
 }
@@ -221,7 +236,7 @@ int PageTable::compact() {
     for (int s = 0; s < seqs; s++)
         for (int j = 0, m = held(s); j < m; j++) fill[row(s)[j]] = std::max(fill[row(s)[j]], blocks_of(s, j));
     copies.clear();
-    slots_valid = false;
+    runs_valid = false;
     if (moves.empty()) return 0;
     for (PageCopy &c : moves) {
         c.blocks = fill[c.src];

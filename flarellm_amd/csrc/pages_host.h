@@ -17,6 +17,13 @@ struct PageCopy {
     int src, dst, blocks;
 };
 
+// Consecutive tokens in one 32-slot block: tokens token .. token + count - 1 of a call in
+// slots slot .. of block page * (page_size / 32) + i.
+struct PageRun {
+    int block, token;
+    short slot, count;
+};
+
 // Pages, their reference counts and the sequences' page lists.  Every call
 // checks its arguments before it changes anything: a call that fails leaves the
 // state as it was.
@@ -27,8 +34,9 @@ struct PageTable {
     std::vector<int> len;    // tokens of each sequence
     std::vector<int> ref;    // sequences that hold a page
     std::vector<PageCopy> copies;  // of the last call
-    std::vector<int> slots;        // page * page_size + slot of every token of the last extend
-    bool slots_valid = false;      // no other call since
+    std::vector<PageRun> runs;     // where the last extend's tokens go
+    int tokens = 0;                // how many
+    bool runs_valid = false;       // no other call since
     uint64_t version = 1;          // changes with the tables and lengths
     std::string error;
 
@@ -40,6 +48,8 @@ struct PageTable {
     int extend(const int32_t *s, const int32_t *counts, int n);
     int compact();
 
+    // appends the runs of tokens [from, to) of a sequence, as tokens `token` .. of a call
+    void add_runs(int s, int from, int to, int token, std::vector<PageRun> &out) const;
     int held(int s) const { return (len[s] + page_size - 1) / page_size; }
     int *row(int s) { return table.data() + (size_t)s * max_pages; }
     const int *row(int s) const { return table.data() + (size_t)s * max_pages; }

@@ -2,6 +2,8 @@
 // their sequences, and the stores, reads and copies of pages.
 #pragma once
 
+#include <type_traits>
+
 #include "bgemm_pack.h"
 #include "pages_args.h"
 
@@ -842,51 +844,121 @@ __global__ __launch_bounds__(256) void k_pages_join(PageJoinArgs a) {
     if (e < a.heads * D) *(pf4_t *)(a.out + (size_t)j.query * a.heads * D + e) = pf4_t{y[0] * il, y[1] * il, y[2] * il, y[3] * il};
 }
 
-// f32 rows into their slots: a thread takes 32 channels of K or V of one token,
-// layer and kv head
+__device__ __forceinline__ PageRun pg_run(const PageRuns &r, int i) { return r.list ? r.list[i] : r.some[i]; }
+// A value as the cache holds it
+template <int FMT>
+using PgElem = std::conditional_t<FMT == FL_KV_F32, float, std::conditional_t<FMT == FL_KV_F16, uint16_t, int8_t>>;
+
+// f32 rows into the slots of a block: a workgroup takes the tokens of one run, one kv head
+// and layer.  A thread has 4 channels of a token; V is turned in LDS, so that a full block
+// leaves in pieces of 16 bytes and a part of one in consecutive slots.  Bound by the memory
+// (a thread for 32 channels with 32 scattered stores took 39 us for 2209 tokens of 8 x 128 in
+// 8 bits, this ..).  grid (runs, kv heads, layers)
 template <int FMT, int D>
-__global__ __launch_bounds__(256) void k_pages_write(PageWriteArgs a, PageSlots slots) {
-    constexpr int NB = D / 32;
-    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-    const long long total = (long long)a.layers * a.n * a.pool.nkv * NB * 2;
-    if (i >= total) return;
-    const int isv = (int)(i & 1), b = (int)(i >> 1) % NB;
-    long long j = (i >> 1) / NB;
-    const int kvh = (int)(j % a.pool.nkv);
-    j /= a.pool.nkv;
-    const int t = (int)(j % a.n), l = (int)(j / a.n);
-    const int at = slots.list ? slots.list[t] : slots.some[t], page = at / a.pool.P, slot = at % a.pool.P;
-    const float *x = (isv ? a.v : a.k) + ((long long)l * a.n + t) * a.stride + kvh * D + 32 * b;
-    const size_t head = ((size_t)(a.layer0 + l) * a.pool.pages + page) * a.pool.nkv + kvh;
-    const size_t base = isv ? head * a.pool.P * D + ((size_t)(slot >> 5) * D + 32 * b) * 32 + (slot & 31)
-                            : (head * a.pool.P + slot) * D + 32 * b;
-    const int step = isv ? 32 : 1;
-    void *o = isv ? a.pool.v : a.pool.k;
-    if constexpr (FMT == FL_KV_Q8) {
-        float amax = 0.0f;
-        for (int e = 0; e < 32; e++) amax = fmaxf(amax, fabsf(x[e]));
-        float d, id;
-        pg_q8_scale(amax, d, id);
-        for (int e = 0; e < 32; e++) ((int8_t *)o)[base + (size_t)e * step] = q8_code(x[e] * id);
-        (isv ? a.pool.vs : a.pool.ks)[(head * a.pool.P + slot) * NB + b] = f2h(d);
+__global__ __launch_bounds__(256) void k_pages_write(PageWriteArgs a, PageRuns runs) {
+    using E = PgElem<FMT>;
+    constexpr int TR = D / 4, PAD = 36;  // threads of a row; elements between V's channels in LDS
+    __shared__ __align__(16) E vt[D * PAD];
+    const PageRun run = pg_run(runs, blockIdx.x);
+    const int kvh = blockIdx.y, layer = blockIdx.z;
+    const int page = run.block / a.pool.per, slot0 = 32 * (run.block - page * a.pool.per);
+    const size_t head = ((size_t)(a.layer0 + layer) * a.pool.pages + page) * a.pool.nkv + kvh;
+    E *kb = (E *)a.pool.k + (head * a.pool.P + slot0) * D, *vb = (E *)a.pool.v + (head * a.pool.P + slot0) * D;
+    uint16_t *ks = a.pool.ks + (head * a.pool.P + slot0) * (D / 32), *vs = a.pool.vs + (head * a.pool.P + slot0) * (D / 32);
+    const int c = threadIdx.x % TR * 4;
+    for (int i = threadIdx.x / TR; i < 2 * run.count; i += 256 / TR) {
+        const int r = i >> 1, isv = i & 1, slot = run.slot + r;
+        const float *x = (isv ? a.v : a.k) + ((long long)layer * a.n + run.token + r) * a.stride + kvh * D + c;
+        float y[4] = {x[0], x[1], x[2], x[3]};
+        E e[4];
+        if constexpr (FMT == FL_KV_Q8) {
+            float amax = fmaxf(fmaxf(fabsf(y[0]), fabsf(y[1])), fmaxf(fabsf(y[2]), fabsf(y[3])));
+#pragma unroll
+            for (int m = 1; m < 8; m <<= 1) amax = fmaxf(amax, __shfl_xor(amax, m, 64));  // 8 threads: 32 channels
+            float d, id;
+            pg_q8_scale(amax, d, id);
+#pragma unroll
+            for (int k = 0; k < 4; k++) e[k] = q8_code(y[k] * id);
+            if (c % 32 == 0) (isv ? vs : ks)[slot * (D / 32) + c / 32] = f2h(d);
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                if constexpr (FMT == FL_KV_F32) e[k] = y[k];
+                else e[k] = f2h(y[k]);
+            }
+        }
+        if (isv) {
+#pragma unroll
+            for (int k = 0; k < 4; k++) vt[(c + k) * PAD + r] = e[k];
+        } else {
+            struct alignas(4 * sizeof(E)) E4 {
+                E x[4];
+            };
+            *(E4 *)(kb + slot * D + c) = E4{{e[0], e[1], e[2], e[3]}};
+        }
+    }
+    __syncthreads();
+    if (run.count == 32) {
+        constexpr int N = 4;  // elements of a piece
+        struct alignas(N * sizeof(E)) EN {
+            E x[N];
+        };
+        for (int i = threadIdx.x; i < D * 32 / N; i += 256)
+            ((EN *)vb)[i] = *(const EN *)(vt + (i / (32 / N)) * PAD + i % (32 / N) * N);
     } else {
-        for (int e = 0; e < 32; e++) {
-            if constexpr (FMT == FL_KV_F32) ((float *)o)[base + (size_t)e * step] = x[e];
-            else ((uint16_t *)o)[base + (size_t)e * step] = f2h(x[e]);
+        for (int i = threadIdx.x; i < D * run.count; i += 256) {
+            const int d = i / run.count, r = i - d * run.count;
+            vb[d * 32 + run.slot + r] = vt[d * PAD + r];
         }
     }
 }
 
-// The values of slots, as f32 rows: a thread per (token, kv head, channel)
+// The values of runs of slots, as f32 rows: a workgroup takes one run and kv head; a thread
+// has 4 channels of a token's K, then 4 slots of a channel's V, turned in LDS.  grid (runs,
+// kv heads)
 template <int FMT, int D>
-__global__ __launch_bounds__(256) void k_pages_read(PageReadArgs a) {
-    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (i >= (long long)a.n * a.pool.nkv * D) return;
-    const int d = (int)(i % D), kvh = (int)(i / D % a.pool.nkv), t = (int)(i / D / a.pool.nkv);
-    const int at = a.slots[t], page = at / a.pool.P, slot = at % a.pool.P;
+__global__ __launch_bounds__(256) void k_pages_read(PageReadArgs a, PageRuns runs) {
+    using E = PgElem<FMT>;
+    constexpr int TR = D / 4, PAD = D + 1;
+    struct alignas(4 * sizeof(E)) E4 {
+        E x[4];
+    };
+    __shared__ float vt[32 * PAD];
+    const PageRun run = pg_run(runs, blockIdx.x);
+    const int kvh = blockIdx.y;
+    const int page = run.block / a.pool.per, slot0 = 32 * (run.block - page * a.pool.per);
     const size_t head = ((size_t)a.layer * a.pool.pages + page) * a.pool.nkv + kvh;
-    if (a.k) a.k[i] = pg_k<FMT, D>(a.pool, head, slot, d);
-    if (a.v) a.v[i] = pg_v<FMT, D>(a.pool, head, slot, d);
+    const E *kb = (const E *)a.pool.k + (head * a.pool.P + slot0) * D, *vb = (const E *)a.pool.v + (head * a.pool.P + slot0) * D;
+    const uint16_t *ks = a.pool.ks + (head * a.pool.P + slot0) * (D / 32), *vs = a.pool.vs + (head * a.pool.P + slot0) * (D / 32);
+    const size_t row = (size_t)a.pool.nkv * D;
+    auto value = [&](E x, const uint16_t *s, int slot, int d) -> float {
+        if constexpr (FMT == FL_KV_F32) return x;
+        else if constexpr (FMT == FL_KV_F16) return h2f(x);
+        else return (float)x * h2f(s[slot * (D / 32) + (d >> 5)]);
+    };
+    const int c = threadIdx.x % TR * 4;
+    if (a.k)
+        for (int r = threadIdx.x / TR; r < run.count; r += 256 / TR) {
+            const int slot = run.slot + r;
+            const E4 x = *(const E4 *)(kb + slot * D + c);
+            float *o = a.k + (size_t)(run.token + r) * row + kvh * D + c;
+#pragma unroll
+            for (int k = 0; k < 4; k++) o[k] = value(x.x[k], ks, slot, c + k);
+        }
+    if (!a.v) return;
+    for (int i = threadIdx.x; i < D * 8; i += 256) {
+        const int d = i >> 3, s = (i & 7) * 4;
+        const E4 x = *(const E4 *)(vb + d * 32 + s);
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+            if (s + k >= run.slot && s + k < run.slot + run.count) vt[(s + k - run.slot) * PAD + d] = value(x.x[k], vs, s + k, d);
+    }
+    __syncthreads();
+    for (int r = threadIdx.x / TR; r < run.count; r += 256 / TR) {
+        float *o = a.v + (size_t)(run.token + r) * row + kvh * D + c;
+#pragma unroll
+        for (int k = 0; k < 4; k++) o[k] = vt[r * PAD + c + k];
+    }
 }
 
 // Blocks of pages to other pages: grid (copies, layers * kv heads); `unit` bytes of
