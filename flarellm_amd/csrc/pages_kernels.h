@@ -23,19 +23,39 @@ __device__ __forceinline__ pf16_t pg_mfma_w(pu4_t a, pu4_t b, pf16_t c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(ph8_t, a), __builtin_bit_cast(ph8_t, b), c, 0, 0, 0);
 }
 
+// Multiply-adds of f32 with binary16 halves of a register (H: the high one), exact products
+// and one rounding: a * b + c as f32, and a * b (+ or - c) rounded to binary16 into a half of d.
+template <int H>
+__device__ __forceinline__ float pg_fma_mix(float a, uint32_t b, float c) {
+    float d;
+    if constexpr (H) asm("v_fma_mix_f32 %0, %1, %2, %3 op_sel:[0,1,0] op_sel_hi:[0,1,0]" : "=v"(d) : "v"(a), "v"(b), "v"(c));
+    else asm("v_fma_mix_f32 %0, %1, %2, %3 op_sel_hi:[0,1,0]" : "=v"(d) : "v"(a), "v"(b), "v"(c));
+    return d;
+}
+// x - hi of two floats and their high parts, as binary16
+__device__ __forceinline__ uint32_t pg_rest2(float x0, float x1, uint32_t hi) {
+    uint32_t d;
+    asm("v_fma_mixlo_f16 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(d) : "v"(hi), "v"(x0));
+    asm("v_fma_mixhi_f16 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "+v"(d) : "v"(hi), "v"(x1));
+    return d;
+}
+// Products of two floats with the halves of s, in two binary16 parts
+__device__ __forceinline__ void pg_mul_split2(float x0, float x1, uint32_t s, uint32_t &hi, uint32_t &lo) {
+    uint32_t h, l;
+    asm("v_fma_mixlo_f16 %0, %1, %2, 0 op_sel_hi:[0,1,0]" : "=v"(h) : "v"(x0), "v"(s));
+    asm("v_fma_mixhi_f16 %0, %1, %2, 0 op_sel:[0,1,0] op_sel_hi:[0,1,0]" : "+v"(h) : "v"(x1), "v"(s));
+    asm("v_fma_mixlo_f16 %0, %1, %2, -%3 op_sel_hi:[0,1,1]" : "=v"(l) : "v"(x0), "v"(s), "v"(h));
+    asm("v_fma_mixhi_f16 %0, %1, %2, -%3 op_sel:[0,1,1] op_sel_hi:[0,1,1]" : "+v"(l) : "v"(x1), "v"(s), "v"(h));
+    hi = h;
+    lo = l;
+}
+
 // 8 floats as two binary16 parts (round toward zero, then the rest)
 __device__ __forceinline__ void pg_split(const float *x, pu4_t &hi, pu4_t &lo) {
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        const auto h = __builtin_amdgcn_cvt_pkrtz(x[2 * i], x[2 * i + 1]);
-        hi[i] = __builtin_bit_cast(uint32_t, h);
-        // x minus its high part, exactly, in one instruction each (a conversion and a
-        // subtraction otherwise)
-        float a, b;
-        asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(a) : "v"(hi[i]), "v"(x[2 * i]));
-        asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(b) : "v"(hi[i]), "v"(x[2 * i + 1]));
-        const auto l = __builtin_amdgcn_cvt_pkrtz(a, b);
-        lo[i] = __builtin_bit_cast(uint32_t, l);
+        hi[i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x[2 * i], x[2 * i + 1]));
+        lo[i] = pg_rest2(x[2 * i], x[2 * i + 1], hi[i]);
     }
 }
 
@@ -186,17 +206,8 @@ template <int D>
 struct PgBlock<FL_KV_Q8, D> {
     static constexpr int QP = D / 32 * 2;
     pu2_t k[2][D / 32], v[D / 16];
-    uint16_t ks[8][D / 32], vs[8][D / 32];  // scales of slots 8 g + 0..7
+    pu4_t ks[D / 32], vs[D / 32];  // scales of slots 8 g + 0..7: value i of [slot][D / 32]
 
-    __device__ __forceinline__ void load_s(const uint16_t *b, uint16_t (*s)[D / 32]) {
-        // 8 slots' scales are contiguous
-#pragma unroll
-        for (int i = 0; i < D / 32; i++) {
-            const pu4_t w = ((const pu4_t *)b)[i];
-#pragma unroll
-            for (int j = 0; j < 8; j++) s[(8 * i + j) / (D / 32)][(8 * i + j) % (D / 32)] = (uint16_t)(w[j >> 1] >> (16 * (j & 1)));
-        }
-    }
     __device__ __forceinline__ void load_k(const PagePool &p, size_t head, int slot, int m, int g) {
         const int8_t *b = (const int8_t *)p.k + (head * p.P + slot) * D;
 #pragma unroll
@@ -204,20 +215,27 @@ struct PgBlock<FL_KV_Q8, D> {
 #pragma unroll
             for (int c = 0; c < D / 32; c++)
                 k[t][c] = *(const pu2_t *)(b + (8 * (m >> 2) + 4 * t + (m & 3)) * D + 32 * c + 8 * g);
-        load_s(p.ks + (head * p.P + slot + 8 * g) * (D / 32), ks);
+        const pu4_t *s = (const pu4_t *)(p.ks + (head * p.P + slot + 8 * g) * (D / 32));
+#pragma unroll
+        for (int i = 0; i < D / 32; i++) ks[i] = s[i];
     }
     __device__ __forceinline__ void load_v(const PagePool &p, size_t head, int slot, int m, int g) {
         const int8_t *b = (const int8_t *)p.v + (head * p.P + slot) * D;
 #pragma unroll
         for (int c = 0; c < D / 16; c++) v[c] = *(const pu2_t *)(b + (16 * c + m) * 32 + 8 * g);
-        load_s(p.vs + (head * p.P + slot + 8 * g) * (D / 32), vs);
+        const pu4_t *s = (const pu4_t *)(p.vs + (head * p.P + slot + 8 * g) * (D / 32));
+#pragma unroll
+        for (int i = 0; i < D / 32; i++) vs[i] = s[i];
     }
     // (codes are finite: only the scales of slots without a token must not meet a zero)
     __device__ __forceinline__ void clip_v(int n, int g) {
 #pragma unroll
-        for (int i = 0; i < 8; i++)
+        for (int i = 0; i < D / 32; i++)
 #pragma unroll
-            for (int c = 0; c < D / 32; c++) vs[i][c] = 8 * g + i < n ? vs[i][c] : (uint16_t)0;
+            for (int j = 0; j < 4; j++) {
+                const int s0 = 8 * g + (8 * i + 2 * j) / (D / 32), s1 = 8 * g + (8 * i + 2 * j + 1) / (D / 32);
+                vs[i][j] &= (s0 < n ? 0xFFFFu : 0u) | (s1 < n ? 0xFFFF0000u : 0u);
+            }
     }
     static __device__ __forceinline__ void make_q(const float *q, float mul, int g, pu4_t *o) {
         PgBlock<FL_KV_F16, D>::make_q(q, mul, g, o);
@@ -232,18 +250,29 @@ struct PgBlock<FL_KV_Q8, D> {
                 pf4_t d = pg_mfma_h(a, q[2 * c + 1], pf4_t{0, 0, 0, 0});
                 d = pg_mfma_h(a, q[2 * c], d);
 #pragma unroll
-                for (int i = 0; i < 4; i++) s[t][i] = __builtin_fmaf(d[i], h2f(ks[4 * t + i][c]), s[t][i]);
+                for (int i = 0; i < 4; i++) {
+                    const int at = (4 * t + i) * (D / 32) + c;  // (even D / 32: its parity is c's)
+                    s[t][i] = (c & 1) ? pg_fma_mix<1>(d[i], ks[at >> 3][(at & 7) >> 1], s[t][i])
+                                      : pg_fma_mix<0>(d[i], ks[at >> 3][(at & 7) >> 1], s[t][i]);
+                }
             }
         }
     }
     __device__ __forceinline__ void add_pv(const float *p, int, pf4_t *o) const {
 #pragma unroll
         for (int c = 0; c < D / 32; c++) {
-            float x[8];
-#pragma unroll
-            for (int j = 0; j < 8; j++) x[j] = p[j] * h2f(vs[j][c]);
             pu4_t hi, lo;
-            pg_split(x, hi, lo);
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                // the scales of two neighbouring slots, side by side
+                const int a0 = 2 * j * (D / 32) + c, a1 = a0 + D / 32;
+                const uint32_t w0 = vs[a0 >> 3][(a0 & 7) >> 1], w1 = vs[a1 >> 3][(a1 & 7) >> 1];
+                const uint32_t s = __builtin_amdgcn_perm(w1, w0, (c & 1) ? 0x07060302u : 0x05040100u);
+                uint32_t h, l;
+                pg_mul_split2(p[2 * j], p[2 * j + 1], s, h, l);
+                hi[j] = h;
+                lo[j] = l;
+            }
 #pragma unroll
             for (int u = 0; u < 2; u++) {
                 const pu4_t a = pg_bytes(v[2 * c + u]);
@@ -853,7 +882,7 @@ using PgElem = std::conditional_t<FMT == FL_KV_F32, float, std::conditional_t<FM
 // and layer.  A thread has 4 channels of a token; V is turned in LDS, so that a full block
 // leaves in pieces of 16 bytes and a part of one in consecutive slots.  Bound by the memory
 // (a thread for 32 channels with 32 scattered stores took 39 us for 2209 tokens of 8 x 128 in
-// 8 bits, this ..).  grid (runs, kv heads, layers)
+// 8 bits, this 9.2).  grid (runs, kv heads, layers)
 template <int FMT, int D>
 __global__ __launch_bounds__(256) void k_pages_write(PageWriteArgs a, PageRuns runs) {
     using E = PgElem<FMT>;
@@ -970,11 +999,23 @@ static __global__ __launch_bounds__(256) void k_pages_copy(PagePool p, PageCopie
     const size_t from = (((size_t)layer * p.pages + x.src) * p.nkv + kvh) * per;
     const size_t to = (((size_t)layer * p.pages + x.dst) * p.nkv + kvh) * per;
     const int n = x.blocks * unit / 16, ns = x.blocks * sunit / 16;
-    for (int i = threadIdx.x; i < n; i += 256) {
-        const pu4_t k = ((const pu4_t *)((const char *)p.k + from * unit))[i];
-        const pu4_t v = ((const pu4_t *)((const char *)p.v + from * unit))[i];
-        ((pu4_t *)((char *)p.k + to * unit))[i] = k;
-        ((pu4_t *)((char *)p.v + to * unit))[i] = v;
+    // U pieces of K and of V of a thread in flight together: 63 copies of 96 tokens of 32 layers
+    // x 8 x 128, binary16, 186 us one by one, 150 by two, 141 so
+    constexpr int U = 8;
+    for (int i = threadIdx.x; i < n; i += 256 * U) {
+        pu4_t x[2 * U];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int j = min(i + 256 * u, n - 1);
+            x[u] = ((const pu4_t *)((const char *)p.k + from * unit))[j];
+            x[U + u] = ((const pu4_t *)((const char *)p.v + from * unit))[j];
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            if (i + 256 * u >= n) break;
+            ((pu4_t *)((char *)p.k + to * unit))[i + 256 * u] = x[u];
+            ((pu4_t *)((char *)p.v + to * unit))[i + 256 * u] = x[U + u];
+        }
     }
     for (int i = threadIdx.x; i < ns; i += 256) {
         ((pu4_t *)((char *)p.ks + to * sunit))[i] = ((const pu4_t *)((const char *)p.ks + from * sunit))[i];

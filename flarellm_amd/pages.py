@@ -63,6 +63,7 @@ class PagedKv:
         #: the backend's stream: with it as the current one, calls need no events
         self.stream = torch.cuda.ExternalStream(backend.stream, device=self.device)
         self._stream = self.stream.cuda_stream
+        self._current, self._index = torch._C._cuda_getCurrentRawStream, self.device.index
         self._row = (kv_heads, head_dim)
         self._before, self._behind = torch.cuda.Event(), torch.cuda.Event()  # (kept: making one costs 10 us)
         # the memory may be what earlier work of the current stream still uses
@@ -94,11 +95,10 @@ class PagedKv:
 
     def _enqueue(self, fn, *args):
         """_call behind the current torch stream's work, and before what follows there."""
+        if self._current(self._index) == self._stream:
+            return self._call(fn, *args)
         import torch
 
-        current = torch._C._cuda_getCurrentRawStream(self.device.index)
-        if current == self._stream:
-            return self._call(fn, *args)
         current = torch.cuda.current_stream(self.device)
         self._before.record(current)
         self.stream.wait_event(self._before)
@@ -112,7 +112,7 @@ class PagedKv:
         """A float32 tensor on this device whose last dimensions are `shape`, without gaps between them."""
         import torch
 
-        if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.device != self.device:
+        if not isinstance(t, torch.Tensor) or t.dtype is not torch.float32 or t.device != self.device:
             raise ValueError(f"{what}: a float32 tensor on {self.device}")
         n = len(shape)
         if t.shape[-n:] != shape:
