@@ -270,10 +270,11 @@ PageRuns runs_of(const std::vector<PageRun> &v, const DevBuf &dev) {
 
 // Costs fitted to measured calls (a block of 32 tokens of D = 128: 0.7 us where the memory
 // bounds it, 1.1 for 128 rows).
-const PageForms &forms_of(const fl_pages *p) {
-    static const PageForms f16 = {3, {16, 64, 128}, 512, {1, 1, 1.6f}, 6, 8, 256};
-    static const PageForms other = {2, {16, 32, 0}, 512, {2, 3, 0}, 6, 4, 512};
-    return p->cfg.kv_format == FL_KV_F16 ? f16 : other;
+PageForms forms_of(const fl_pages *p) {
+    const int fmt = p->cfg.kv_format, D = p->cfg.head_dim, cus = 256;
+    const int fill = 2 * cus;  // (4 a CU, which D = 64 has the registers for, 22 us against 19 for 32768 tokens of 8 x 64, binary16)
+    if (fmt == FL_KV_F16) return {3, {16, 64, 128}, fill, {1, 1, 1.6f}, 6, 8, cus};
+    return {2, {16, 32}, fill, {2, 3}, 6, 4, cus * page_waves(fmt, D, 2)};
 }
 
 // The plan of these queries, on the device.

@@ -31,6 +31,14 @@ struct PageAttnArgs {
     float *out;            // [n][heads * D]
 };
 
+// Waves per SIMD, so workgroups of 4 waves per CU, that the attention kernel's registers
+// allow (without a bound the compiler takes accumulation registers as well, and half of
+// them).  forms: 1 (up to 16 rows) or 2 (up to 32; f32 of D = 128 with two waves and
+// its queries in LDS 66 us against 55 for 8 queries of 32768 tokens, 8 bits 31 against 33).
+constexpr int page_waves(int fmt, int D, int forms) {
+    return forms == 1 ? (D == 64 ? 4 : fmt == FL_KV_F16 ? 3 : 2) : fmt == FL_KV_Q8 ? (D == 64 ? 3 : 2) : D == 64 ? 2 : 1;
+}
+
 struct PageJoinArgs {
     const PageJoin *joins;
     const int *units;

@@ -23,39 +23,38 @@ __device__ __forceinline__ pf16_t pg_mfma_w(pu4_t a, pu4_t b, pf16_t c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(ph8_t, a), __builtin_bit_cast(ph8_t, b), c, 0, 0, 0);
 }
 
-// Multiply-adds of f32 with binary16 halves of a register (H: the high one), exact products
-// and one rounding: a * b + c as f32, and a * b (+ or - c) rounded to binary16 into a half of d.
-template <int H>
-__device__ __forceinline__ float pg_fma_mix(float a, uint32_t b, float c) {
-    float d;
-    if constexpr (H) asm("v_fma_mix_f32 %0, %1, %2, %3 op_sel:[0,1,0] op_sel_hi:[0,1,0]" : "=v"(d) : "v"(a), "v"(b), "v"(c));
-    else asm("v_fma_mix_f32 %0, %1, %2, %3 op_sel_hi:[0,1,0]" : "=v"(d) : "v"(a), "v"(b), "v"(c));
-    return d;
+// Mixed multiply-adds of f32 and binary16 (v_fma_mix*: exact products, one rounding), as
+// expressions that the compiler selects them from: written as assembly, nothing would keep
+// them the distance from matrix products, exponentials and half-register writes that
+// these need.  The multiplier of -1 is opaque, or the compiler makes two instructions of it.
+typedef _Float16 ph2_t __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ float pg_minus_one() {
+    float m = -1.0f;
+    asm("" : "+v"(m));
+    return m;
 }
-// x - hi of two floats and their high parts, as binary16
-__device__ __forceinline__ uint32_t pg_rest2(float x0, float x1, uint32_t hi) {
-    uint32_t d;
-    asm("v_fma_mixlo_f16 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(d) : "v"(hi), "v"(x0));
-    asm("v_fma_mixhi_f16 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "+v"(d) : "v"(hi), "v"(x1));
-    return d;
+__device__ __forceinline__ float pg_fma_mix(float a, uint32_t b, int half, float c) {
+    return __builtin_fmaf(a, (float)__builtin_bit_cast(ph2_t, b)[half], c);
 }
 // Products of two floats with the halves of s, in two binary16 parts
 __device__ __forceinline__ void pg_mul_split2(float x0, float x1, uint32_t s, uint32_t &hi, uint32_t &lo) {
-    uint32_t h, l;
-    asm("v_fma_mixlo_f16 %0, %1, %2, 0 op_sel_hi:[0,1,0]" : "=v"(h) : "v"(x0), "v"(s));
-    asm("v_fma_mixhi_f16 %0, %1, %2, 0 op_sel:[0,1,0] op_sel_hi:[0,1,0]" : "+v"(h) : "v"(x1), "v"(s));
-    asm("v_fma_mixlo_f16 %0, %1, %2, -%3 op_sel_hi:[0,1,1]" : "=v"(l) : "v"(x0), "v"(s), "v"(h));
-    asm("v_fma_mixhi_f16 %0, %1, %2, -%3 op_sel:[0,1,1] op_sel_hi:[0,1,1]" : "+v"(l) : "v"(x1), "v"(s), "v"(h));
-    hi = h;
-    lo = l;
+    const ph2_t w = __builtin_bit_cast(ph2_t, s);
+    const ph2_t h = {(_Float16)(x0 * (float)w[0]), (_Float16)(x1 * (float)w[1])};
+    const ph2_t l = {(_Float16)__builtin_fmaf(x0, (float)w[0], -(float)h[0]),
+                     (_Float16)__builtin_fmaf(x1, (float)w[1], -(float)h[1])};
+    hi = __builtin_bit_cast(uint32_t, h);
+    lo = __builtin_bit_cast(uint32_t, l);
 }
 
 // 8 floats as two binary16 parts (round toward zero, then the rest)
 __device__ __forceinline__ void pg_split(const float *x, pu4_t &hi, pu4_t &lo) {
+    const float minus = pg_minus_one();
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        hi[i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x[2 * i], x[2 * i + 1]));
-        lo[i] = pg_rest2(x[2 * i], x[2 * i + 1], hi[i]);
+        const auto h = __builtin_amdgcn_cvt_pkrtz(x[2 * i], x[2 * i + 1]);
+        hi[i] = __builtin_bit_cast(uint32_t, h);
+        lo[i] = __builtin_bit_cast(uint32_t, ph2_t{(_Float16)__builtin_fmaf((float)h[0], minus, x[2 * i]),
+                                                   (_Float16)__builtin_fmaf((float)h[1], minus, x[2 * i + 1])});
     }
 }
 
@@ -179,25 +178,33 @@ struct PgBlock<FL_KV_F16, D> {
             pg_split(x, o[2 * c], o[2 * c + 1]);
         }
     }
-    __device__ __forceinline__ void scores(const pu4_t *q, int, pf4_t *s) const {
+    // of NT tiles of 16 rows: what is made of k and v is made once
+    template <int NT, typename Q>
+    __device__ __forceinline__ void scores(const Q &q, pf4_t (*s)[2]) const {
 #pragma unroll
-        for (int t = 0; t < 2; t++) {
-            pf4_t lo = {0, 0, 0, 0}, hi = {0, 0, 0, 0};
+        for (int n = 0; n < NT; n++)
 #pragma unroll
-            for (int c = 0; c < D / 32; c++) {
-                lo = pg_mfma_h(k[t][c], q[2 * c + 1], lo);
-                hi = pg_mfma_h(k[t][c], q[2 * c], hi);
+            for (int t = 0; t < 2; t++) {
+                pf4_t lo = {0, 0, 0, 0}, hi = {0, 0, 0, 0};
+#pragma unroll
+                for (int c = 0; c < D / 32; c++) {
+                    lo = pg_mfma_h(k[t][c], q(n, 2 * c + 1), lo);
+                    hi = pg_mfma_h(k[t][c], q(n, 2 * c), hi);
+                }
+                s[n][t] = hi + lo;
             }
-            s[t] = hi + lo;
-        }
     }
-    __device__ __forceinline__ void add_pv(const float *p, int, pf4_t *o) const {
-        pu4_t hi, lo;
-        pg_split(p, hi, lo);
+    template <int NT>
+    __device__ __forceinline__ void add_pv(const float (*p)[8], pf4_t (*o)[D / 16]) const {
 #pragma unroll
-        for (int c = 0; c < D / 16; c++) {
-            o[c] = pg_mfma_h(v[c], lo, o[c]);
-            o[c] = pg_mfma_h(v[c], hi, o[c]);
+        for (int n = 0; n < NT; n++) {
+            pu4_t hi, lo;
+            pg_split(p[n], hi, lo);
+#pragma unroll
+            for (int c = 0; c < D / 16; c++) {
+                o[n][c] = pg_mfma_h(v[c], lo, o[n][c]);
+                o[n][c] = pg_mfma_h(v[c], hi, o[n][c]);
+            }
         }
     }
 };
@@ -240,44 +247,55 @@ struct PgBlock<FL_KV_Q8, D> {
     static __device__ __forceinline__ void make_q(const float *q, float mul, int g, pu4_t *o) {
         PgBlock<FL_KV_F16, D>::make_q(q, mul, g, o);
     }
-    __device__ __forceinline__ void scores(const pu4_t *q, int, pf4_t *s) const {
+    template <int NT, typename Q>
+    __device__ __forceinline__ void scores(const Q &q, pf4_t (*s)[2]) const {
 #pragma unroll
         for (int t = 0; t < 2; t++) {
-            s[t] = pf4_t{0, 0, 0, 0};
+#pragma unroll
+            for (int n = 0; n < NT; n++) s[n][t] = pf4_t{0, 0, 0, 0};
 #pragma unroll
             for (int c = 0; c < D / 32; c++) {
                 const pu4_t a = pg_bytes(k[t][c]);
-                pf4_t d = pg_mfma_h(a, q[2 * c + 1], pf4_t{0, 0, 0, 0});
-                d = pg_mfma_h(a, q[2 * c], d);
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int at = (4 * t + i) * (D / 32) + c;  // (even D / 32: its parity is c's)
-                    s[t][i] = (c & 1) ? pg_fma_mix<1>(d[i], ks[at >> 3][(at & 7) >> 1], s[t][i])
-                                      : pg_fma_mix<0>(d[i], ks[at >> 3][(at & 7) >> 1], s[t][i]);
+                for (int n = 0; n < NT; n++) {
+                    pf4_t d = pg_mfma_h(a, q(n, 2 * c + 1), pf4_t{0, 0, 0, 0});
+                    d = pg_mfma_h(a, q(n, 2 * c), d);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const int at = (4 * t + i) * (D / 32) + c;  // (even D / 32: its parity is c's)
+                        s[n][t][i] = pg_fma_mix(d[i], ks[at >> 3][(at & 7) >> 1], c & 1, s[n][t][i]);
+                    }
                 }
             }
         }
     }
-    __device__ __forceinline__ void add_pv(const float *p, int, pf4_t *o) const {
+    template <int NT>
+    __device__ __forceinline__ void add_pv(const float (*p)[8], pf4_t (*o)[D / 16]) const {
 #pragma unroll
         for (int c = 0; c < D / 32; c++) {
-            pu4_t hi, lo;
+            pu4_t hi[NT], lo[NT];
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 // the scales of two neighbouring slots, side by side
                 const int a0 = 2 * j * (D / 32) + c, a1 = a0 + D / 32;
                 const uint32_t w0 = vs[a0 >> 3][(a0 & 7) >> 1], w1 = vs[a1 >> 3][(a1 & 7) >> 1];
                 const uint32_t s = __builtin_amdgcn_perm(w1, w0, (c & 1) ? 0x07060302u : 0x05040100u);
-                uint32_t h, l;
-                pg_mul_split2(p[2 * j], p[2 * j + 1], s, h, l);
-                hi[j] = h;
-                lo[j] = l;
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+                    uint32_t h, l;
+                    pg_mul_split2(p[n][2 * j], p[n][2 * j + 1], s, h, l);
+                    hi[n][j] = h;
+                    lo[n][j] = l;
+                }
             }
 #pragma unroll
             for (int u = 0; u < 2; u++) {
                 const pu4_t a = pg_bytes(v[2 * c + u]);
-                o[2 * c + u] = pg_mfma_h(a, lo, o[2 * c + u]);
-                o[2 * c + u] = pg_mfma_h(a, hi, o[2 * c + u]);
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+                    o[n][2 * c + u] = pg_mfma_h(a, lo[n], o[n][2 * c + u]);
+                    o[n][2 * c + u] = pg_mfma_h(a, hi[n], o[n][2 * c + u]);
+                }
             }
         }
     }
@@ -315,24 +333,47 @@ struct PgBlock<FL_KV_F32, D> {
 #pragma unroll
             for (int j = 0; j < 4; j++) o[c][j] = __float_as_uint(q[16 * c + 4 * g + j] * mul);
     }
-    __device__ __forceinline__ void scores(const pu4_t *q, int, pf4_t *s) const {
+    template <int NT, typename Q>
+    __device__ __forceinline__ void scores(const Q &q, pf4_t (*s)[2]) const {
 #pragma unroll
-        for (int t = 0; t < 2; t++) {
-            s[t] = pf4_t{0, 0, 0, 0};
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+                s[n][t] = pf4_t{0, 0, 0, 0};
+#pragma unroll
+                for (int c = 0; c < D / 16; c++) {
+                    const pu4_t w = q(n, c);
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        s[n][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[t][c][j], __uint_as_float(w[j]), s[n][t], 0, 0, 0);
+                }
+            }
+    }
+    template <int NT>
+    __device__ __forceinline__ void add_pv(const float (*p)[8], pf4_t (*o)[D / 16]) const {
+#pragma unroll
+        for (int n = 0; n < NT; n++)
 #pragma unroll
             for (int c = 0; c < D / 16; c++)
 #pragma unroll
-                for (int j = 0; j < 4; j++)
-                    s[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[t][c][j], __uint_as_float(q[c][j]), s[t], 0, 0, 0);
-        }
+                for (int j = 0; j < 8; j++)
+                    o[n][c] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[c][j >> 2][j & 3], p[n][j], o[n][c], 0, 0, 0);
     }
-    __device__ __forceinline__ void add_pv(const float *p, int, pf4_t *o) const {
-#pragma unroll
-        for (int c = 0; c < D / 16; c++)
-#pragma unroll
-            for (int j = 0; j < 8; j++)
-                o[c] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[c][j >> 2][j & 3], p[j], o[c], 0, 0, 0);
-    }
+};
+
+constexpr bool pg_q_in_lds(int fmt, int D, int nt) { return fmt == FL_KV_Q8 && nt == 2 && D == 128; }
+// The query operands of NT tiles: registers, or (LDS) the same of all waves in LDS, for the
+// forms whose registers would not do for two waves a SIMD.
+template <int NT, int QP, bool LDS>
+struct PgQ {
+    pu4_t r[NT][QP];
+    __device__ __forceinline__ const pu4_t &operator()(int n, int i) const { return r[n][i]; }
+};
+template <int NT, int QP>
+struct PgQ<NT, QP, true> {
+    const pu4_t *base;
+    int at;  // the lane's
+    __device__ __forceinline__ pu4_t operator()(int n, int i) const { return base[at + (n * QP + i) * 64]; }
 };
 
 // Where an item's blocks are.  Its page numbers go through the scalar cache, asked for a
@@ -479,6 +520,7 @@ __device__ __forceinline__ void pg_join_row(const PageAttnArgs &a, const PageIte
 template <int FMT, int D, int NT, int NW>
 __device__ __forceinline__ void pg_narrow(const PageAttnArgs &a, const PageItem &it, int kvh, float *lds, int *bad) {
     using Block = PgBlock<FMT, D>;
+    constexpr bool QL = pg_q_in_lds(FMT, D, NT);
     constexpr int QP = Block::QP, DT = D / 16, LROW = D + 4;
     const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -500,7 +542,8 @@ __device__ __forceinline__ void pg_narrow(const PageAttnArgs &a, const PageItem 
 
     pg_stage_q<D, LROW, 64 * NW>(a, it, kvh, lds);
     __syncthreads();
-    pu4_t q[NT][QP];
+    PgQ<NT, QP, QL> q;
+    pu4_t *ql = (pu4_t *)(lds + NW * 16 * LROW);  // behind the join's
     float c[NT];
     int seen[NT];
 #pragma unroll
@@ -518,7 +561,20 @@ __device__ __forceinline__ void pg_narrow(const PageAttnArgs &a, const PageItem 
                 for (int j = 0; j < 8; j++) x = fmaxf(x, fabsf(qp[32 * k + 8 * g + j]));
             pg_q_scale(pg_max16(x), mul, c[n]);
         }
-        Block::make_q(qp, mul, g, q[n]);
+        if constexpr (QL) {
+            if (wave != n) continue;
+            pu4_t w[QP];
+            Block::make_q(qp, mul, g, w);
+#pragma unroll
+            for (int i = 0; i < QP; i++) ql[(n * QP + i) * 64 + lane] = w[i];
+        } else {
+            Block::make_q(qp, mul, g, q.r[n]);
+        }
+    }
+    if constexpr (QL) {
+        q.base = ql;
+        q.at = lane;
+        __syncthreads();
     }
     pf4_t o[NT][DT];
     float m_run[NT], l_run[NT];
@@ -533,8 +589,8 @@ __device__ __forceinline__ void pg_narrow(const PageAttnArgs &a, const PageItem 
     for (int b = wave; b < nb; b += NW) {
         const int tok = it.slot0 + 32 * b;  // first token of the block
         pf4_t s[NT][2];
-#pragma unroll
-        for (int n = 0; n < NT; n++) blk.scores(q[n], g, s[n]);
+        if constexpr (QL) asm volatile("" : "+v"(q.at));  // read again, not kept in registers
+        blk.template scores<NT>(q, s);
         const size_t head = (layer_pages + page) * nkv + kvh;
         const int slot = walk.slot(b1);
         blk.load_k(a.pool, head, slot, m, g);
@@ -548,6 +604,7 @@ __device__ __forceinline__ void pg_narrow(const PageAttnArgs &a, const PageItem 
                     if (tok + 8 * g + j >= min(seen[n], it.slot1)) s[n][j >> 2][j & 3] = -INFINITY;
             if (tok + 32 > it.slot1) blk.clip_v(it.slot1 - tok, g);
         }
+        float p[NT][8];
 #pragma unroll
         for (int n = 0; n < NT; n++) {
             float x = s[n][0][0];
@@ -566,14 +623,13 @@ __device__ __forceinline__ void pg_narrow(const PageAttnArgs &a, const PageItem 
             }
             // (a row that has seen no token yet has scores of -Inf alone, and p = 0)
             const float off = m_run[n] == -INFINITY ? -INFINITY : kPageShift<FMT> - m_run[n];
-            float p[8];
 #pragma unroll
             for (int j = 0; j < 8; j++) {
-                p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][j >> 2][j & 3], c[n], off));
-                l_run[n] += p[j];
+                p[n][j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][j >> 2][j & 3], c[n], off));
+                l_run[n] += p[n][j];
             }
-            blk.add_pv(p, g, o[n]);
         }
+        blk.template add_pv<NT>(p, o);
         blk.load_v(a.pool, head, slot, m, g);
     }
 
@@ -785,8 +841,8 @@ __device__ __forceinline__ void pg_wide(const PageAttnArgs &a, const PageItem &i
 
 // Items of up to 16 rows (FORMS = 1), or up to 32: 4 waves.
 template <int FMT, int D, int FORMS>
-__global__ __launch_bounds__(256) void k_pages_attn(PageAttnArgs a) {
-    __shared__ __align__(16) float lds[4 * 16 * (D + 4)];
+__global__ __launch_bounds__(256, page_waves(FMT, D, FORMS)) void k_pages_attn(PageAttnArgs a) {
+    __shared__ __align__(16) float lds[4 * 16 * (D + 4) + (pg_q_in_lds(FMT, D, FORMS) ? FORMS * PgBlock<FMT, D>::QP * 256 : 0)];
     __shared__ int bad;
     const int kvh = blockIdx.x % a.pool.nkv;
     const PageItem it = pg_item(a, blockIdx.x / a.pool.nkv);
