@@ -36,25 +36,24 @@ __device__ __forceinline__ float pg_minus_one() {
 __device__ __forceinline__ float pg_fma_mix(float a, uint32_t b, int half, float c) {
     return __builtin_fmaf(a, (float)__builtin_bit_cast(ph2_t, b)[half], c);
 }
-// Products of two floats with the halves of s, in two binary16 parts
-__device__ __forceinline__ void pg_mul_split2(float x0, float x1, uint32_t s, uint32_t &hi, uint32_t &lo) {
-    const ph2_t w = __builtin_bit_cast(ph2_t, s);
-    const ph2_t h = {(_Float16)(x0 * (float)w[0]), (_Float16)(x1 * (float)w[1])};
-    const ph2_t l = {(_Float16)__builtin_fmaf(x0, (float)w[0], -(float)h[0]),
-                     (_Float16)__builtin_fmaf(x1, (float)w[1], -(float)h[1])};
+// 2 floats as two binary16 parts: round toward zero, then the rest.  (The first part is
+// rounded by an instruction of its own: of (_Float16)(x * y) the compiler makes v_fma_mixlo's
+// one rounding in one place and two in another, and the parts no longer fit together.)
+__device__ __forceinline__ void pg_split2(float x0, float x1, float minus, uint32_t &hi, uint32_t &lo) {
+    const auto h = __builtin_amdgcn_cvt_pkrtz(x0, x1);
     hi = __builtin_bit_cast(uint32_t, h);
-    lo = __builtin_bit_cast(uint32_t, l);
+    lo = __builtin_bit_cast(uint32_t, ph2_t{(_Float16)__builtin_fmaf((float)h[0], minus, x0),
+                                            (_Float16)__builtin_fmaf((float)h[1], minus, x1)});
 }
-
-// 8 floats as two binary16 parts (round toward zero, then the rest)
+// 8 floats
 __device__ __forceinline__ void pg_split(const float *x, pu4_t &hi, pu4_t &lo) {
     const float minus = pg_minus_one();
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        const auto h = __builtin_amdgcn_cvt_pkrtz(x[2 * i], x[2 * i + 1]);
-        hi[i] = __builtin_bit_cast(uint32_t, h);
-        lo[i] = __builtin_bit_cast(uint32_t, ph2_t{(_Float16)__builtin_fmaf((float)h[0], minus, x[2 * i]),
-                                                   (_Float16)__builtin_fmaf((float)h[1], minus, x[2 * i + 1])});
+        uint32_t h, l;
+        pg_split2(x[2 * i], x[2 * i + 1], minus, h, l);
+        hi[i] = h;
+        lo[i] = l;
     }
 }
 
@@ -122,8 +121,9 @@ __device__ __forceinline__ void pg_q8_scale(float amax, float &scale, float &fac
 // A row's O and sum are kept relative to a maximum that follows its scores only when one
 // is over it by 2^kPageLag (nearly every block has a new maximum of some row, and
 // bringing O to it is a third of a block's vector work).  p is kept times 2^kPageShift
-// where its parts are binary16: at most 2^15, and what its low part loses below 2^-24 is
-// 2^-33 of the largest p.
+// where its parts are binary16: at most 2^15, and what its low part loses below 2^-14, if
+// products take smaller numbers for 0, is 2^-23 of the largest p.  In 8 bits the parts are
+// those of p times V's scale, so the maximum is over the scores with the scale's exponent.
 constexpr float kPageLag = 6.0f;
 template <int FMT>
 constexpr float kPageShift = FMT == FL_KV_F32 ? 0.0f : 9.0f;
@@ -178,6 +178,7 @@ struct PgBlock<FL_KV_F16, D> {
             pg_split(x, o[2 * c], o[2 * c + 1]);
         }
     }
+    __device__ __forceinline__ float v_exponent() const { return 0.0f; }
     // of NT tiles of 16 rows: what is made of k and v is made once
     template <int NT, typename Q>
     __device__ __forceinline__ void scores(const Q &q, pf4_t (*s)[2]) const {
@@ -244,6 +245,16 @@ struct PgBlock<FL_KV_Q8, D> {
                 vs[i][j] &= (s0 < n ? 0xFFFFu : 0u) | (s1 < n ? 0xFFFF0000u : 0u);
             }
     }
+    // a power of two over the scales of the lane's slots
+    __device__ __forceinline__ float v_exponent() const {
+        typedef uint16_t u2 __attribute__((ext_vector_type(2)));
+        u2 m = {0, 0};
+#pragma unroll
+        for (int i = 0; i < D / 32; i++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) m = __builtin_elementwise_max(m, __builtin_bit_cast(u2, vs[i][j]));
+        return (float)(max((int)m[0], (int)m[1]) >> 10) - 14.0f;
+    }
     static __device__ __forceinline__ void make_q(const float *q, float mul, int g, pu4_t *o) {
         PgBlock<FL_KV_F16, D>::make_q(q, mul, g, o);
     }
@@ -271,6 +282,7 @@ struct PgBlock<FL_KV_Q8, D> {
     }
     template <int NT>
     __device__ __forceinline__ void add_pv(const float (*p)[8], pf4_t (*o)[D / 16]) const {
+        const float minus = pg_minus_one();
 #pragma unroll
         for (int c = 0; c < D / 32; c++) {
             pu4_t hi[NT], lo[NT];
@@ -283,7 +295,7 @@ struct PgBlock<FL_KV_Q8, D> {
 #pragma unroll
                 for (int n = 0; n < NT; n++) {
                     uint32_t h, l;
-                    pg_mul_split2(p[n][2 * j], p[n][2 * j + 1], s, h, l);
+                    pg_split2(pg_fma_mix(p[n][2 * j], s, 0, 0.0f), pg_fma_mix(p[n][2 * j + 1], s, 1, 0.0f), minus, h, l);
                     hi[n][j] = h;
                     lo[n][j] = l;
                 }
@@ -327,6 +339,7 @@ struct PgBlock<FL_KV_F32, D> {
 #pragma unroll
             for (int j = 0; j < 8; j++) v[c][j >> 2][j & 3] = 8 * g + j < n ? v[c][j >> 2][j & 3] : 0.0f;
     }
+    __device__ __forceinline__ float v_exponent() const { return 0.0f; }
     static __device__ __forceinline__ void make_q(const float *q, float mul, int g, pu4_t *o) {
 #pragma unroll
         for (int c = 0; c < D / 16; c++)
@@ -605,12 +618,13 @@ __device__ __forceinline__ void pg_narrow(const PageAttnArgs &a, const PageItem 
             if (tok + 32 > it.slot1) blk.clip_v(it.slot1 - tok, g);
         }
         float p[NT][8];
+        const float ve = blk.v_exponent();
 #pragma unroll
         for (int n = 0; n < NT; n++) {
             float x = s[n][0][0];
 #pragma unroll
             for (int j = 1; j < 8; j++) x = fmaxf(x, s[n][j >> 2][j & 3]);
-            x = pg_max16(x) * c[n];
+            x = pg_max16(__builtin_fmaf(x, c[n], ve));
             if (__any(x > m_run[n] + kPageLag)) {
                 const float mn = fmaxf(m_run[n], x);
                 const float al = m_run[n] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m_run[n] - mn);

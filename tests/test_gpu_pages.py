@@ -194,6 +194,22 @@ def test_several_queries_of_a_sequence(backend, fmt, queries):
     t.check([int(s) for s in seqs], [int(rng.integers(0, n[s] + 1)) for s in seqs])
 
 
+@pytest.mark.parametrize("fmt", ["f32", "f16", "q8"])
+@pytest.mark.parametrize("heads,kv_heads,D,forks", [(8, 2, 64, 1), (8, 2, 64, 8), (16, 2, 128, 20), (4, 2, 128, 8)])
+@pytest.mark.parametrize("size", [1.0, 1e-3, 300.0])
+def test_nothing_is_lost_on_the_whole(backend, fmt, heads, kv_heads, D, forks, size):
+    """The error of all values together: roundings of 2^-24 each, independent of each
+    other, D of them in a score of size 1 (16 x 2^-24 at most), as many again of its
+    weight and of the sum: 2^-19 of the result's 2-norm.  For V of any size."""
+    t = Twin(backend, fmt, heads, kv_heads, D, 64, 80, seqs=32, seed=forks)
+    for n in (300, 2500):
+        k, v = (t.rng.standard_normal((1, n, kv_heads, D)).astype(np.float32) for _ in "kv")
+        t.extend([0], [n], (k, (v * size).astype(np.float32)))
+    t.fork([0] * (forks - 1), range(1, forks))
+    got, want, _ = t.attend(list(range(forks)))
+    assert np.linalg.norm(got - want) <= 2.0**-19 * np.linalg.norm(want)
+
+
 def test_the_same_as_the_contiguous_cache(backend):
     """One sequence: the attention of fl_gqa_from_cache over the same rows."""
     from flarellm_amd.synth import ModelSpec
