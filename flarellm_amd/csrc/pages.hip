@@ -23,6 +23,7 @@ struct Stage {
     bool used = false;
 };
 constexpr int kStages = 4;
+constexpr int kPageMaxQueries = 1 << 20;
 constexpr int kPageMaxGroup = 32;  // query heads per kv head: the rows of the largest form of every cache
 
 struct DevBuf {
@@ -503,7 +504,7 @@ int fl_pages_attention(fl_pages *p, int layer, const float *q, size_t q_stride, 
     const int D = p->cfg.head_dim, nkv = p->cfg.num_kv_heads;
     if (num_heads < 1 || num_heads % nkv) return fail(p, FL_E_INVALID, "%d heads over %d kv heads", num_heads, nkv);
     if (num_heads / nkv > kPageMaxGroup) return fail(p, FL_E_UNSUPPORTED, "%d query heads per kv head", num_heads / nkv);
-    if (n < 0) return fail(p, FL_E_INVALID, "%d queries", n);
+    if (n < 0 || n > kPageMaxQueries) return fail(p, FL_E_INVALID, "%d queries (up to %d)", n, kPageMaxQueries);
     if (n == 0) return 0;
     if (!q || !out || !seqs || !seen) return fail(p, FL_E_INVALID, "null argument");
     if ((uintptr_t)q % 4 || (uintptr_t)out % 16) return fail(p, FL_E_INVALID, "queries or result are not aligned");
@@ -526,6 +527,7 @@ int fl_pages_attention(fl_pages *p, int layer, const float *q, size_t q_stride, 
     a.ml = a.part + (size_t)l.num_units * num_heads * D;
     a.out = out;
     a.items = (const PageItem *)d;
+    if ((long long)l.items.size() * nkv > 0x7FFFFFFFll) return fail(p, FL_E_INVALID, "too many queries at once");
     if (!l.items.empty())
         PGCHK(p, (hipError_t)with_form(p->cfg.kv_format, D, LaunchAttn{p->stream, a, (int)l.items.size(), l.wide}));
     if (!l.joins.empty()) {

@@ -46,7 +46,7 @@ class PagedKv:
         self.lib = backend.lib
         self.layers, self.pages, self.page_size = layers, pages, page_size
         self.kv_heads, self.head_dim, self.kv_format = kv_heads, head_dim, kv_format
-        self.max_seqs, self.max_len = max_seqs, max_len or pages * page_size
+        self.max_seqs, self.max_len = max_seqs, max_len or min(pages * page_size, 1 << 24)
         cfg = PagesConfig(layers, kv_heads, head_dim, kv_format, pages, page_size, max_seqs, self.max_len)
         check(self.lib.fl_pages_bytes(C.byref(cfg), None, None))
         self.device = torch.device("cuda", self.lib.fl_ctx_device(backend.ctx))

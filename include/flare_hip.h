@@ -421,7 +421,8 @@ int fl_pages_extend(fl_pages *p, const int32_t *seqs, const int32_t *counts, int
 /* Stores keys and values of the last fl_pages_extend's tokens, sequence by sequence
  * in its order, in `layers` layers from `layer` on: device f32, token i of the l-th
  * of them at (l * tokens + i) * row_stride, num_kv_heads * head_dim values.  (The
- * other calls that change sequences end this: FL_E_STATE.) */
+ * other calls that change sequences end this: FL_E_STATE.  Slots hold what they held
+ * until they are stored to.) */
 int fl_pages_write(fl_pages *p, int layer, int layers, const float *k, const float *v, size_t row_stride);
 /* Moves pages so that those in use are the ones of lowest index; *moved (may be
  * NULL): how many were moved. */
@@ -436,7 +437,8 @@ int fl_pages_read(fl_pages *p, int layer, const int32_t *seqs, const int32_t *st
  * of sequence seqs[i] (host arrays; a sequence may have any number of queries), each
  * as grouped_query_attention_from_gpu_cache (model.rs:311).  seen[i] = 0 gives zeros.
  * A page that several of the call's sequences hold is read once for all of them.  out
- * [n][num_heads * head_dim] f32, 16-byte aligned.  Up to 32 query heads per kv head. */
+ * [n][num_heads * head_dim] f32, 16-byte aligned, apart from q.  Up to 32 query heads
+ * per kv head and 2^20 queries.  A workspace for partial results stays with the pool. */
 int fl_pages_attention(fl_pages *p, int layer, const float *q, size_t q_stride, const int32_t *seqs,
                        const int32_t *seen, int n, int num_heads, float *out);
 /* Tokens of a sequence, tokens that fl_pages_write stores, free pages of the pool

@@ -348,6 +348,49 @@ def test_a_batch_from_prompt_to_answers(backend):
     assert t.kv.free_pages == 64 and used < 4 * (137 + 40) // 32
 
 
+@pytest.mark.parametrize("fmt,heads,kv_heads,page", [("q8", 32, 1, 4096), ("f32", 64, 2, 128), ("f16", 64, 2, 4096)])
+def test_the_largest_groups_and_pages(backend, fmt, heads, kv_heads, page):
+    t = Twin(backend, fmt, heads, kv_heads, 64, page, 8 if page > 1000 else 40, seqs=5, max_len=4200, fill=float("nan"), seed=page)
+    t.extend([0, 1], [700, 3])
+    t.fork([0], [2])
+    t.extend([2, 0], [1, 2])
+    t.check([0, 1, 2, 2, 3], [702, 3, 701, 65, 0])
+    t.check_rows()
+
+
+def test_odd_strides(backend):
+    """Rows of odd widths, several layers at once."""
+    t = Twin(backend, "q8", 4, 2, 64, 32, 20, layers=3)
+    k, v = (torch.randn(3, 37, 131, device="cuda")[:, :, 2:130].view(3, 37, 2, 64) for _ in "kv")
+    t.kv.extend([1, 2], [30, 7])
+    t.kv.write(k[1:], v[1:], layer=1)
+    t.kv.write(k[0], v[0])
+    t.rows[1], t.rows[2] = ([stored("q8", x[:, s].cpu().numpy().copy()) for x in (k, v)] for s in (slice(0, 30), slice(30, 37)))
+    t.check_rows()
+    q = torch.randn(5, 259, device="cuda")[:, 1:257].view(5, 4, 64)
+    seqs, seen = [1, 2, 1, 2, 1], [30, 7, 1, 2, 29]
+    for l in range(3):
+        want, tol = t.want(q.cpu().numpy(), seqs, seen, l)
+        assert (np.abs(t.kv.attention(q, seqs, seen, layer=l).cpu().numpy() - want) <= tol).all()
+
+
+@pytest.mark.parametrize("fmt", ["f16", "q8"])
+def test_offsets_past_32_bits(backend, fmt):
+    """Pages whose elements begin past 2^32."""
+    page, nkv, D = 128, 8, 128
+    high = (1 << 32) // (page * nkv * D) + 50
+    t = Twin(backend, fmt, 16, nkv, D, page, high + 8, seqs=4, max_len=high * page)
+    t.kv.extend([3], [high * page])  # (its rows are not looked at)
+    t.extend([0], [200])
+    assert t.kv.tables()[0][0] == high
+    t.fork([0], [1])
+    t.extend([1, 0], [3, 70])
+    t.check([0, 1, 0], [270, 203, 5])
+    t.check_rows()
+    del t
+    torch.cuda.empty_cache()
+
+
 def test_two_pools_at_once(backend):
     """Pools share the backend's stream, not their workspaces or plans."""
     a = Twin(backend, "f16", 8, 2, 64, 64, 60, seed=1)
@@ -433,3 +476,15 @@ def test_capture_is_refused(backend):
     torch.cuda.synchronize()
     assert x.tolist() == [1.0] * 4 and t.kv.length(0) == 70
     t.check([0])
+    # the capture of another stream, which the backend's joins
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        x += 1
+        with pytest.raises(FlareError, match="captured"):
+            t.kv.attention(q, [0], out=out)
+        x += 1
+    for i in range(3):
+        g.replay()
+        torch.cuda.synchronize()
+        assert x.tolist() == [3.0 + 2 * i] * 4
+        t.check([0])
