@@ -24,6 +24,7 @@ struct Stage {
 };
 constexpr int kStages = 4;
 constexpr int kPageMaxQueries = 1 << 20;
+constexpr int kMaxGrid = (1 << 24) - 1;  // workgroups of 256 threads along x: a grid's threads are counted in 32 bits
 constexpr int kPageMaxGroup = 32;  // query heads per kv head: the rows of the largest form of every cache
 
 struct DevBuf {
@@ -99,7 +100,7 @@ int check_config(const fl_pages_config *c) {
         return fail(nullptr, FL_E_INVALID, "page size %d (a multiple of 32 up to 4096)", c->page_size);
     if (c->num_layers < 1 || c->num_kv_heads < 1 || (long long)c->num_layers * c->num_kv_heads > 65535)
         return fail(nullptr, FL_E_INVALID, "%d layers of %d kv heads", c->num_layers, c->num_kv_heads);
-    if (c->num_pages < 1 || (long long)c->num_pages * c->page_size > 0x7FFFFFFFll)
+    if (c->num_pages < 1 || c->num_pages > kMaxGrid || (long long)c->num_pages * c->page_size > 0x7FFFFFFFll)
         return fail(nullptr, FL_E_INVALID, "%d pages of %d tokens", c->num_pages, c->page_size);
     if (c->max_seqs < 1 || c->max_seq_len < 1 || c->max_seq_len > (1 << 24) ||
         (long long)c->max_seqs * ((c->max_seq_len + c->page_size - 1) / c->page_size) > (1ll << 28))
@@ -135,9 +136,9 @@ int ensure(fl_pages *p, DevBuf &b, size_t bytes) {
     return 0;
 }
 
-// Pinned memory for `bytes` that go to the device with send().
-int stage_for(fl_pages *p, size_t bytes, char **host) {
-    Stage &s = p->stages[p->stage];
+// Room for `bytes` in the stage of the next send() but `ahead`.
+int stage_room(fl_pages *p, int ahead, size_t bytes) {
+    Stage &s = p->stages[(p->stage + ahead) % kStages];
     if (s.used) PGCHK(p, hipEventSynchronize(s.done));
     s.used = false;
     if (s.cap < bytes) {
@@ -152,7 +153,13 @@ int stage_for(fl_pages *p, size_t bytes, char **host) {
         s.cap = cap;
     }
     if (!s.done) PGCHK(p, hipEventCreateWithFlags(&s.done, hipEventDisableTiming));
-    *host = s.host;
+    return 0;
+}
+
+// Pinned memory for `bytes` that go to the device with send().
+int stage_for(fl_pages *p, size_t bytes, char **host) {
+    PGTRY(stage_room(p, 0, bytes));
+    *host = p->stages[p->stage].host;
     return 0;
 }
 
@@ -171,6 +178,11 @@ int upload(fl_pages *p, DevBuf &b, const void *data, size_t bytes) {
     PGTRY(stage_for(p, bytes, &h));
     memcpy(h, data, bytes);
     return send(p, b.p, bytes);
+}
+
+// Room for a list of up to n copies, before the bookkeeping that makes it.
+int copies_room(fl_pages *p, int ahead, long long n) {
+    return n > kInlineCopies ? stage_room(p, ahead, (size_t)n * sizeof(PageCopy)) : 0;
 }
 
 int run_copies(fl_pages *p) {
@@ -403,20 +415,25 @@ int fl_pages_truncate(fl_pages *p, const int32_t *seqs, const int32_t *lens, int
 }
 
 int fl_pages_copy(fl_pages *p, const int32_t *src, const int32_t *dst, int n) {
-    if (p && p->ctx) PGTRY(check_stream(p));
-    PGTRY(on_table(p, [&](PageTable &t) { return t.copy(src, dst, n); }));
-    if (!p->ctx) return 0;
+    if (!p) return fail(p, FL_E_INVALID, "null pages");
+    if (!p->ctx) return on_table(p, [&](PageTable &t) { return t.copy(src, dst, n); });
+    PGTRY(check_stream(p));
     OnDevice on(p);
+    PGTRY(copies_room(p, 0, std::min((long long)std::max(n, 0) * p->t.max_pages, (long long)p->t.free_pages)));
+    PGTRY(on_table(p, [&](PageTable &t) { return t.copy(src, dst, n); }));
     return run_copies(p);
 }
 
 int fl_pages_compact(fl_pages *p, int *moved) {
-    if (p && p->ctx) PGTRY(check_stream(p));
+    if (!p) return fail(p, FL_E_INVALID, "null pages");
+    OnDevice on(p);
+    if (p->ctx) {
+        PGTRY(check_stream(p));
+        PGTRY(copies_room(p, 0, std::min(p->t.free_pages, p->cfg.num_pages - p->t.free_pages)));
+    }
     PGTRY(on_table(p, [&](PageTable &t) { return t.compact(); }));
     if (moved) *moved = (int)p->t.copies.size();
-    if (!p->ctx) return 0;
-    OnDevice on(p);
-    return run_copies(p);
+    return p->ctx ? run_copies(p) : 0;
 }
 
 int fl_pages_extend(fl_pages *p, const int32_t *seqs, const int32_t *counts, int n) {
@@ -424,12 +441,21 @@ int fl_pages_extend(fl_pages *p, const int32_t *seqs, const int32_t *counts, int
     if (!p->ctx) return on_table(p, [&](PageTable &t) { return t.extend(seqs, counts, n); });
     PGTRY(check_stream(p));
     OnDevice on(p);
-    // room for the runs first: nothing fails behind the bookkeeping
+    // Room for the lists first: no allocation fails behind the bookkeeping.  A call that fails
+    // in it leaves the runs of the one before, and these may still be written.
     long long most = 0;
     for (int i = 0; i < n && counts; i++) most += std::min(std::max(counts[i], 0), p->cfg.max_seq_len) / kPageBlock + 2;
     most = std::min(most, (long long)p->cfg.num_pages * p->pool.per + n);
-    if (most > kInlineRuns) PGTRY(ensure(p, p->d_runs, (size_t)most * sizeof(PageRun)));
-    PGTRY(on_table(p, [&](PageTable &t) { return t.extend(seqs, counts, n); }));
+    if (most > kMaxGrid) return fail(p, FL_E_INVALID, "too many tokens at once");
+    DevBuf more;
+    const size_t bytes = most > kInlineRuns ? (size_t)most * sizeof(PageRun) : 0;
+    int rc = copies_room(p, bytes ? 1 : 0, n);
+    if (!rc && bytes) rc = stage_room(p, 0, bytes);
+    if (!rc && bytes > p->d_runs.cap) rc = ensure(p, more, std::max(bytes, 2 * p->d_runs.cap));
+    if (!rc) rc = on_table(p, [&](PageTable &t) { return t.extend(seqs, counts, n); });
+    if (!rc && more.p) std::swap(more, p->d_runs);
+    if (more.p) (void)hipFree(more.p);  // (waits for what reads it)
+    if (rc) return rc;
     const auto &r = p->t.runs;
     if (r.size() > kInlineRuns) PGTRY(upload(p, p->d_runs, r.data(), r.size() * sizeof(PageRun)));
     return run_copies(p);
@@ -489,6 +515,8 @@ int fl_pages_read(fl_pages *p, int layer, const int32_t *seqs, const int32_t *st
     }));
     if (runs.empty()) return 0;
     if (!k && !v) return fail(p, FL_E_INVALID, "null keys and values");
+    if (((uintptr_t)k | (uintptr_t)v) % 4) return fail(p, FL_E_INVALID, "keys or values are not aligned");
+    if (runs.size() > kMaxGrid) return fail(p, FL_E_INVALID, "too many tokens at once");
     OnDevice on(p);
     if (runs.size() > kInlineRuns) PGTRY(upload(p, p->d_read, runs.data(), runs.size() * sizeof(PageRun)));
     PageReadArgs a{p->pool, k, v, layer};
@@ -503,13 +531,17 @@ int fl_pages_attention(fl_pages *p, int layer, const float *q, size_t q_stride, 
     PGTRY(check_layers(p, layer, 1));
     const int D = p->cfg.head_dim, nkv = p->cfg.num_kv_heads;
     if (num_heads < 1 || num_heads % nkv) return fail(p, FL_E_INVALID, "%d heads over %d kv heads", num_heads, nkv);
-    if (num_heads / nkv > kPageMaxGroup) return fail(p, FL_E_UNSUPPORTED, "%d query heads per kv head", num_heads / nkv);
+    if (num_heads / nkv > kPageMaxGroup || num_heads > 65535)
+        return fail(p, FL_E_UNSUPPORTED, "%d query heads, %d per kv head", num_heads, num_heads / nkv);
     if (n < 0 || n > kPageMaxQueries) return fail(p, FL_E_INVALID, "%d queries (up to %d)", n, kPageMaxQueries);
     if (n == 0) return 0;
     if (!q || !out || !seqs || !seen) return fail(p, FL_E_INVALID, "null argument");
     if ((uintptr_t)q % 4 || (uintptr_t)out % 16) return fail(p, FL_E_INVALID, "queries or result are not aligned");
     if (q_stride < (size_t)num_heads * D) return fail(p, FL_E_INVALID, "queries of %d values %zu apart", num_heads * D, q_stride);
     PGTRY(check_stream(p));
+    const uintptr_t q0 = (uintptr_t)q, o0 = (uintptr_t)out;
+    if (q0 < o0 + (size_t)n * num_heads * D * 4 && o0 < q0 + ((n - 1) * q_stride + (size_t)num_heads * D) * 4)
+        return fail(p, FL_E_INVALID, "queries and result overlap");
     OnDevice on(p);
     PGTRY(make_plan(p, seqs, seen, n, num_heads));
     const PagePlan &l = p->plan;
@@ -527,7 +559,7 @@ int fl_pages_attention(fl_pages *p, int layer, const float *q, size_t q_stride, 
     a.ml = a.part + (size_t)l.num_units * num_heads * D;
     a.out = out;
     a.items = (const PageItem *)d;
-    if ((long long)l.items.size() * nkv > 0x7FFFFFFFll) return fail(p, FL_E_INVALID, "too many queries at once");
+    if ((long long)l.items.size() * nkv > (l.wide && p->cfg.kv_format == FL_KV_F16 ? kMaxGrid / 2 : kMaxGrid)) return fail(p, FL_E_INVALID, "too many queries at once");
     if (!l.items.empty())
         PGCHK(p, (hipError_t)with_form(p->cfg.kv_format, D, LaunchAttn{p->stream, a, (int)l.items.size(), l.wide}));
     if (!l.joins.empty()) {

@@ -13,6 +13,7 @@ namespace fl {
 
 namespace {
 int ceil_div(int a, int b) { return (int)(((long long)a + b - 1) / b); }
+constexpr size_t kMaxOrder = 1 << 26;  // a query once per run that it sees: 0.5 GB, and counts of parts stay in 32 bits
 }  // namespace
 
 int PageTable::fail(int code, const char *fmt, ...) {
@@ -35,7 +36,7 @@ int PageTable::init(const fl_pages_config &c) {
     table.assign((size_t)seqs * max_pages, -1);
     len.assign(seqs, 0);
     ref.assign(pages, 0);
-    stamp.assign(std::max(seqs, pages), 0);
+    stamp.assign(seqs, 0);
     free_bits.assign((pages + 63) / 64, ~0ull);
     if (pages % 64) free_bits.back() = (1ull << (pages % 64)) - 1;
     return 0;
@@ -367,6 +368,7 @@ int page_plan(PageTable &t, const int32_t *s, const int32_t *seen, int n, int gr
                 if (seen[q] <= from) break;
                 p.order.push_back({q, seen[q]});
             }
+        if (p.order.size() > kMaxOrder) return fail(FL_E_INVALID, "too many queries of too many shared lists at once");
         const int end = e * P, total = (int)p.order.size() - first;
         std::stable_sort(p.order.begin() + first, p.order.end(), [&](const PageQuery &a, const PageQuery &b) {
             return std::min(a.seen, end) > std::min(b.seen, end);

@@ -57,8 +57,8 @@ struct PageTable {
 private:
     std::vector<uint64_t> free_bits;
     int hint = 0;            // no free page below 64 * hint
-    std::vector<int> stamp;  // marks of one call
-    int stamp_now = 0;
+    std::vector<uint64_t> stamp;  // the last call that listed a sequence
+    uint64_t stamp_now = 0;
     int take();
     void drop(int page);
     int fail(int code, const char *fmt, ...) __attribute__((format(printf, 3, 4)));

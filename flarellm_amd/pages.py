@@ -9,7 +9,7 @@ behind one system prompt.
 
 Work is enqueued on the backend's stream.  Calls made with another current torch
 stream order the two streams by events, so tensors go in and come out as with any
-torch operation; no call waits for the GPU.
+torch operation; calls do not wait for the GPU (but where their lists outgrow their memory).
 """
 from __future__ import annotations
 
@@ -86,9 +86,12 @@ class PagedKv:
         except Exception:
             pass
 
-    def _call(self, fn, *args):
+    def _open(self):
         if not self._h or not self._b.ctx:
             raise FlareError("the paged cache or its backend is closed")
+
+    def _call(self, fn, *args):
+        self._open()
         rc = fn(self._h, *args)
         if rc:
             check(rc, self._b.ctx)
@@ -167,11 +170,13 @@ class PagedKv:
     def length(self, seq: int) -> int:
         n = self.lib.fl_pages_len(self._h, seq)
         if n < 0:
+            self._open()
             raise ValueError(f"sequence {seq} of {self.max_seqs}")
         return n
 
     @property
     def free_pages(self) -> int:
+        self._open()
         return self.lib.fl_pages_free_count(self._h)
 
     def tables(self) -> np.ndarray:
@@ -201,7 +206,8 @@ class PagedKv:
         if n == 0:
             return
         layers = k.shape[0] if k.dim() == 4 else 1
-        stride = k.stride(-3) if n > 1 else max(k.stride(-3), self.kv_heads * self.head_dim)
+        row = self.kv_heads * self.head_dim
+        stride = k.stride(-3) if n > 1 else max(k.stride(0), row) if layers > 1 else row
         if layers > 1 and k.stride(0) != n * stride:
             raise ValueError("k and v: gaps between layers")
         self._enqueue(self.lib.fl_pages_write, layer, layers, k.data_ptr(), v.data_ptr(), stride)
@@ -220,7 +226,7 @@ class PagedKv:
 
     def attention(self, q, seqs, seen=None, layer: int = 0, out=None):
         """Attention of queries q [n, heads, head_dim] (RoPE applied; rows may be slices of wider ones): query i
-        over the first seen[i] tokens (all of them) of sequence seqs[i].  -> [n, heads, head_dim]"""
+        over the first seen[i] tokens (all of them) of sequence seqs[i].  -> [n, heads, head_dim] (out: apart from q)"""
         import torch
 
         if not isinstance(q, torch.Tensor) or q.dim() != 3:
@@ -239,7 +245,7 @@ class PagedKv:
             self._rows(out, "out", shape)
             if out.dim() != 3:
                 raise ValueError("out: [n, heads, head_dim]")
-        stride = q.stride(0) if n > 1 else max(q.stride(0), heads * self.head_dim)
+        stride = q.stride(0) if n > 1 else heads * self.head_dim
         self._enqueue(self.lib.fl_pages_attention, layer, q.data_ptr(), stride, seqs.tobytes(), seen.tobytes(), n, heads,
                       out.data_ptr())
         return out

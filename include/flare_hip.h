@@ -385,14 +385,15 @@ int fl_read_tokens(fl_ctx *ctx, int start, int n, uint32_t *out);
  * The bookkeeping is the host's and immediate.  Every call checks its arguments
  * before it changes anything, and one that fails leaves the pool and the sequences
  * as they were (after FL_E_HIP nothing is certain).  What a call does on the device
- * is enqueued on the context's stream, and no call waits for it; none can be
+ * is enqueued on the context's stream, and no call waits for it, but where memory for
+ * its lists grows or the lists of four calls before it are yet to be taken; none can be
  * captured into a graph (FL_E_STATE).  Destroy a pool before its context.  As a
  * context, a pool is not thread-safe. */
 typedef struct fl_pages fl_pages;
 typedef struct {
     int num_layers, num_kv_heads, head_dim; /* head_dim 64 or 128 */
     int kv_format;                          /* FL_KV_F32, FL_KV_F16 or FL_KV_Q8 */
-    int num_pages, page_size;               /* page_size a multiple of 32, up to 4096 */
+    int num_pages, page_size;               /* below 2^24; a multiple of 32, up to 4096 */
     int max_seqs, max_seq_len;              /* sequences 0..max_seqs-1 of up to max_seq_len tokens */
 } fl_pages_config;
 /* Bytes of k (and of v), and of k_scale (and of v_scale; 0 without scales). */

@@ -358,6 +358,36 @@ def test_the_largest_groups_and_pages(backend, fmt, heads, kv_heads, page):
     t.check_rows()
 
 
+def test_an_extend_that_fails_leaves_the_one_before(backend):
+    """Its tokens, in more blocks than go with a launch, may still be stored."""
+    t = Twin(backend, "f16", 4, 1, 64, 32, 300, seqs=8, max_len=9600)
+    x = [torch.randn(5000, 1, 64, device="cuda") for _ in "kv"]
+    t.kv.extend([0, 1], [4500, 500])
+    with pytest.raises(FlareError, match="needed"):
+        t.kv.extend([0, 2], [4800, 9600])
+    with pytest.raises(FlareError):
+        t.kv.extend([2, 2], [9600, 1])
+    t.kv.write(*x)
+    t.rows[0], t.rows[1] = ([stored("f16", r[None, s].cpu().numpy()) for r in x] for s in (slice(0, 4500), slice(4500, 5000)))
+    t.check_rows()
+    t.check([0, 1])
+    t.extend([1, 2], [100, 4300])  # one that outgrows its memory and does not
+    t.check_rows()
+
+
+def test_one_token_of_many_layers(backend):
+    """A token of a [layers, tokens, ..] buffer; a page's last slots."""
+    t = Twin(backend, "f32", 4, 2, 64, 32, 20, layers=4)
+    k, v = (torch.randn(4, 40, 2, 64, device="cuda") for _ in "kv")
+    for i in range(40):
+        t.kv.extend([5], [1])
+        t.kv.write(k[:, i: i + 1], v[:, i: i + 1])
+    t.rows[5] = (k.cpu().numpy(), v.cpu().numpy())
+    t.check_rows()
+    for l in range(4):
+        t.check([5, 5], [40, 33], layer=l)
+
+
 def test_odd_strides(backend):
     """Rows of odd widths, several layers at once."""
     t = Twin(backend, "q8", 4, 2, 64, 32, 20, layers=3)
@@ -452,6 +482,26 @@ def test_refusals(backend):
     kv.close()
     with pytest.raises(FlareError, match="closed"):
         kv.attention(q, [0], [1])
+
+
+def test_queries_and_result_apart(backend):
+    t = Twin(backend, "f16", 8, 2, 64, 32, 10, seqs=4, max_len=100)
+    t.extend([0], [40])
+    x = torch.randn(5, 8, 64, device="cuda")
+    before = x.clone()
+    for q, out in ((x[:2], x[:2]), (x[:2], x[1:3]), (x[1:3], x[:2]), (x[::2], x[2:5])):
+        with pytest.raises(FlareError, match="overlap"):
+            t.kv.attention(q, [0] * q.shape[0], [40] * q.shape[0], out=out)
+    assert torch.equal(x, before)
+    t.kv.attention(x[:2], [0, 0], [40, 7], out=x[2:4])  # side by side
+    want, tol = t.want(before[:2].cpu().numpy(), [0, 0], [40, 7], 0)
+    assert (np.abs(x[2:4].cpu().numpy() - want) <= tol).all() and torch.equal(x[4], before[4])
+    with pytest.raises(FlareError, match="layers"):
+        t.kv.read([0], [0], [1], layer=1)
+    t.kv.close()
+    for call in (lambda: t.kv.free_pages, lambda: t.kv.length(0), t.kv.tables, t.kv.compact):
+        with pytest.raises(FlareError, match="closed"):
+            call()
 
 
 def test_capture_is_refused(backend):

@@ -228,7 +228,7 @@ def test_refusals_leave_everything_as_it_was():
 @pytest.mark.parametrize("change,code", [
     (dict(head_dim=96), UNSUPPORTED), (dict(fmt=L.FL_KV_KIVI2), UNSUPPORTED), (dict(fmt=9), UNSUPPORTED),
     (dict(page_size=48), INVALID), (dict(page_size=0), INVALID), (dict(page_size=8192), INVALID), (dict(pages=0), INVALID),
-    (dict(pages=1 << 26, page_size=64), INVALID), (dict(seqs=0), INVALID), (dict(max_len=0), INVALID),
+    (dict(pages=1 << 26, page_size=64), INVALID), (dict(pages=1 << 24, page_size=32), INVALID), (dict(seqs=0), INVALID), (dict(max_len=0), INVALID),
     (dict(layers=0), INVALID), (dict(kv_heads=0), INVALID), (dict(layers=1 << 12, kv_heads=16), INVALID),
     (dict(seqs=1 << 30), INVALID)])
 def test_bad_configurations(change, code):
