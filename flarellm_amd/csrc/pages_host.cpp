@@ -391,6 +391,8 @@ int page_plan(PageTable &t, const int32_t *s, const int32_t *seen, int n, int gr
     const float *cost = forms.wide_cost;
     const int step = p.wide ? forms.wide_step : 4, least = 8;  // blocks of a step, of a part
     auto whole = [&](long long x) { return (int)((std::max<long long>(x, least) + step - 1) / step * step); };
+    // blocks of a part, of nb in parts of up to `part`
+    auto cut = [&](int nb, int part) { return (ceil_div(nb, ceil_div(nb, part)) + step - 1) / step * step; };
     int part[2] = {longest[0], longest[1]};
     if (!p.wide) {
         // The memory bounds all of them, and a few workgroups a CU keep it busy.
@@ -408,21 +410,28 @@ int page_plan(PageTable &t, const int32_t *s, const int32_t *seen, int n, int gr
         const int machines = std::max(1, forms.wide_slots / kv_heads);
         // joining: a launch and its traffic, in blocks (0.7 us for 16 KB a CU)
         const double even = (double)blocks / machines, join = 6, unit = 8.0 * kv_heads * group * head_dim / 3.5e6;
-        static const double kOf[6] = {0, 1, 0.67, 0.5, 0.34, 0.25};
+        static const double kOf[] = {0, 1, 0.9, 0.8, 0.67, 0.5, 0.34, 0.25, 0.12, 0.06};
+        constexpr int kSome = sizeof kOf / sizeof *kOf;
         double best = 0;
         std::vector<std::pair<float, int>> jobs;  // (time, how many)
         std::vector<float> heap;
-        for (int i = 0; i < 6; i++)
-            for (int j = 0; j < 6; j++) {
-                const int len[2] = {i ? whole((long long)(even * kOf[i])) : longest[0], j ? whole((long long)(even * kOf[j])) : longest[1]};
+        auto of = [&](int i) { return whole((long long)(even * kOf[i])); };
+        auto again = [&](int i) { return i > 1 && of(i) == of(i - 1); };
+        for (int i = 0; i < kSome; i++)
+            for (int j = 0; j < kSome; j++) {
+                if (again(i) || again(j)) continue;
+                const int len[2] = {i ? of(i) : longest[0], j ? of(j) : longest[1]};
                 if ((i && len[0] >= longest[0]) || (j && len[1] >= longest[1])) continue;
                 jobs.clear();
-                double units = 0;
+                double units = 0, sum = 0;
                 for (const Tile &x : tiles) {
-                    const int nb = ceil_div(x.slot1 - x.slot0, kPageBlock), cuts = ceil_div(nb, len[x.form > 1]);
-                    jobs.push_back({ceil_div(nb, cuts) * cost[x.form] + forms.fixed, cuts});
+                    const int nb = ceil_div(x.slot1 - x.slot0, kPageBlock), each = cut(nb, len[x.form > 1]), cuts = ceil_div(nb, each);
+                    jobs.push_back({std::min(each, nb) * cost[x.form] + forms.fixed, cuts});
+                    sum += (double)jobs.back().first * cuts;
                     if (cuts > 1) units += (double)cuts * x.nq;
                 }
+                const double behind = units > 0 ? join + units * unit : 0;
+                if ((i || j) && sum / machines + behind >= best) continue;
                 std::sort(jobs.begin(), jobs.end(), std::greater<>());
                 heap.assign(machines, 0.0f);  // a min-heap of when each machine is free
                 for (auto &w : jobs)
@@ -431,7 +440,7 @@ int page_plan(PageTable &t, const int32_t *s, const int32_t *seen, int n, int gr
                         heap.back() += w.first;
                         std::push_heap(heap.begin(), heap.end(), std::greater<>());
                     }
-                const double time = *std::max_element(heap.begin(), heap.end()) + (units > 0 ? join + units * unit : 0);
+                const double time = *std::max_element(heap.begin(), heap.end()) + behind;
                 if ((i || j) && time >= best) continue;
                 best = time;
                 part[0] = len[0];
@@ -440,8 +449,7 @@ int page_plan(PageTable &t, const int32_t *s, const int32_t *seen, int n, int gr
     }
     std::vector<int> count(n, 0);
     for (const Tile &x : tiles) {
-        const int nb = ceil_div(x.slot1 - x.slot0, kPageBlock), cuts = ceil_div(nb, part[x.form > 1]);
-        const int each = (ceil_div(nb, cuts) + step - 1) / step * step;
+        const int nb = ceil_div(x.slot1 - x.slot0, kPageBlock), each = cut(nb, part[x.form > 1]);
         for (int b = 0; b < nb; b += each) {
             PageItem it{};
             it.q0 = x.q0;
