@@ -46,7 +46,7 @@ struct fl_pages {
     std::vector<int32_t> plan_seqs, plan_seen;
     int plan_heads = 0;
     uint64_t plan_version = 0;
-    size_t plan_order = 0, plan_pages = 0, plan_units = 0, plan_joins = 0;  // offsets
+    size_t plan_order = 0, plan_pages = 0, plan_units = 0, plan_joins = 0, plan_join_of = 0, plan_arrived = 0;  // offsets
     DevBuf d_plan, d_runs, d_read, d_copies, ws;
     Stage stages[kStages];
     int stage = 0;
@@ -232,17 +232,19 @@ struct LaunchAttn {
     int items;
     bool wide;
     template <int FMT, int D>
-    int operator()() const {
+    int operator()() const { return a.arrived ? launch<FMT, D, true>() : launch<FMT, D, false>(); }
+    template <int FMT, int D, bool HERE>
+    int launch() const {
         const dim3 grid((unsigned)(items * a.pool.nkv));
         if (!wide) {
-            hipLaunchKernelGGL((k_pages_attn<FMT, D, 1>), grid, dim3(256), 0, st, a);
+            hipLaunchKernelGGL((k_pages_attn<FMT, D, 1, HERE>), grid, dim3(256), 0, st, a);
         } else if constexpr (FMT == FL_KV_F16) {
             // two steps of K and V, or one and the queries, or the waves' results
             constexpr size_t row = (D + 4) * 4, kv = 8 * 32 * D * 2;
             constexpr size_t lds = std::max({2 * kv, kv + 128 * row, 8 * 32 * row});
-            hipLaunchKernelGGL(k_pages_attn_wide<D>, grid, dim3(512), lds, st, a);
+            hipLaunchKernelGGL((k_pages_attn_wide<D, HERE>), grid, dim3(512), lds, st, a);
         } else {
-            hipLaunchKernelGGL((k_pages_attn<FMT, D, 2>), grid, dim3(256), 0, st, a);
+            hipLaunchKernelGGL((k_pages_attn<FMT, D, 2, HERE>), grid, dim3(256), 0, st, a);
         }
         return (int)hipGetLastError();
     }
@@ -290,6 +292,22 @@ PageForms forms_of(const fl_pages *p) {
     return {2, {16, 32}, fill, {2, 3}, 6, 4, cus * page_waves(fmt, D, 2)};
 }
 
+// Whether the workgroups of the plan's items join its partial results: where the last to
+// arrive reads 8 at most per thread (4 channels of a query and head), in flight together, and
+// they are few (8 answers behind 785 tokens 14.8 us against 17.3 with a launch for them, drafts
+// of 5 sequences 14.4 against 17.0, 21 sequences behind 595 tokens, two times 4 a thread, 15.4
+// against 17.7).  With more it goes over them again and again, past the caches: two times 8 of
+// 4 sequences behind 1774 tokens 19.2 against 17.6, 16 sequences of up to 8000 45.4 against 41.7,
+// 32 in a tree 44 against 24; and stores past the caches cost more than those that
+// stay: 644 queries, 10 MB, 62.2 against 58.5.
+bool joins_here(const fl_pages *p, int heads) {
+    const PagePlan &l = p->plan;
+    const int threads = l.wide && p->cfg.kv_format == FL_KV_F16 ? 512 : 256;
+    const int rows = l.most_queries * (heads / p->cfg.num_kv_heads);
+    const long long rounds = (rows * (p->cfg.head_dim / 4) + threads - 1) / threads;
+    return !l.items.empty() && rounds * l.most_parts <= 8 && (long long)l.num_units * heads * p->cfg.head_dim <= (1 << 18);
+}
+
 // The plan of these queries, on the device.
 int make_plan(fl_pages *p, const int32_t *seqs, const int32_t *seen, int n, int heads) {
     const int group = heads / p->cfg.num_kv_heads;
@@ -316,6 +334,10 @@ int make_plan(fl_pages *p, const int32_t *seqs, const int32_t *seen, int n, int 
     p->plan_pages = place(l.page_ids.size() * sizeof(int));
     p->plan_units = place(l.units.size() * sizeof(int));
     p->plan_joins = place(l.joins.size() * sizeof(PageJoin));
+    p->plan_join_of = place(l.join_of.size() * sizeof(int));
+    p->plan_arrived = bytes;
+    const size_t counts = joins_here(p, heads) ? l.joins.size() * p->cfg.num_kv_heads * sizeof(int) : 0;
+    bytes += counts;
     char *h;
     PGTRY(ensure(p, p->d_plan, bytes));
     PGTRY(ensure(p, p->ws, (size_t)l.num_units * heads * (p->cfg.head_dim + 2) * sizeof(float)));
@@ -328,6 +350,8 @@ int make_plan(fl_pages *p, const int32_t *seqs, const int32_t *seen, int n, int 
     put(p->plan_pages, l.page_ids);
     put(p->plan_units, l.units);
     put(p->plan_joins, l.joins);
+    put(p->plan_join_of, l.join_of);
+    memset(h + p->plan_arrived, 0, counts);
     PGTRY(send(p, p->d_plan.p, bytes));
     p->plan_heads = heads;
     p->plan_version = p->t.version;
@@ -559,10 +583,19 @@ int fl_pages_attention(fl_pages *p, int layer, const float *q, size_t q_stride, 
     a.ml = a.part + (size_t)l.num_units * num_heads * D;
     a.out = out;
     a.items = (const PageItem *)d;
+    const bool here = joins_here(p, num_heads);
+    if (here && !l.joins.empty()) {
+        a.arrived = (int *)(d + p->plan_arrived);
+        a.joins = (const PageJoin *)(d + p->plan_joins);
+        a.units = (const int *)(d + p->plan_units);
+        a.join_of = (const int *)(d + p->plan_join_of);
+        a.njoins = (int)l.joins.size();
+        a.nempty = l.empty;
+    }
     if ((long long)l.items.size() * nkv > (l.wide && p->cfg.kv_format == FL_KV_F16 ? kMaxGrid / 2 : kMaxGrid)) return fail(p, FL_E_INVALID, "too many queries at once");
     if (!l.items.empty())
         PGCHK(p, (hipError_t)with_form(p->cfg.kv_format, D, LaunchAttn{p->stream, a, (int)l.items.size(), l.wide}));
-    if (!l.joins.empty()) {
+    if (!here && !l.joins.empty()) {
         PageJoinArgs j{(const PageJoin *)(d + p->plan_joins), (const int *)(d + p->plan_units), a.part, a.ml, out, num_heads};
         const dim3 grid((unsigned)l.joins.size(), (unsigned)((num_heads * D + 127) / 128));
         if (D == 64) hipLaunchKernelGGL(k_pages_join<64>, grid, dim3(256), 0, p->stream, j);

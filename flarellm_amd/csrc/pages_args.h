@@ -29,6 +29,12 @@ struct PageAttnArgs {
     const int *page_ids;
     float *part, *ml;      // partial results [unit][head][D], [unit][head][2] = (max, sum)
     float *out;            // [n][heads * D]
+    // where the last workgroup to have a part of a query's result joins them (otherwise
+    // arrived is nullptr, and k_pages_join does):
+    int *arrived;          // [join][kv head], zeros between calls
+    const PageJoin *joins;
+    const int *units, *join_of;  // join of a query
+    int njoins, nempty;    // the last nempty of them have no parts
 };
 
 // Waves per SIMD, so workgroups of 4 waves per CU, that the attention kernel's registers

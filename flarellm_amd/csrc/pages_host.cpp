@@ -282,7 +282,7 @@ int page_plan(PageTable &t, const int32_t *s, const int32_t *seen, int n, int gr
     p.page_ids.clear();
     p.units.clear();
     p.joins.clear();
-    p.num_units = 0;
+    p.num_units = p.most_queries = 0;
     const int P = t.page_size;
 
     // the call's sequences, each with its queries (longest first) and pages in view
@@ -473,13 +473,25 @@ int page_plan(PageTable &t, const int32_t *s, const int32_t *seen, int n, int gr
         for (int i = 0; i < it.nq; i++) alone = alone && count[p.order[it.q0 + i].query] == 1;
         it.unit = alone ? -1 : p.num_units;
         if (alone) continue;
+        p.most_queries = std::max(p.most_queries, it.nq);
         for (int i = 0; i < it.nq; i++) joined[p.order[it.q0 + i].query] = 1;
         p.num_units += it.nq;
     }
     for (int i = 0; i < n; i++) first[i + 1] = first[i] + (joined[i] ? count[i] : 0);
     p.units.resize(first[n]);
-    for (int i = 0; i < n; i++)
-        if (joined[i] || !count[i]) p.joins.push_back({i, first[i], joined[i] ? count[i] : 0, 0});
+    p.join_of.assign(n, -1);
+    p.empty = p.most_parts = 0;
+    for (int i = 0; i < n; i++) {
+        if (!joined[i]) continue;
+        p.join_of[i] = (int)p.joins.size();
+        p.joins.push_back({i, first[i], count[i], 0});
+        p.most_parts = std::max(p.most_parts, count[i]);
+    }
+    for (int i = 0; i < n; i++) {
+        if (count[i]) continue;
+        p.joins.push_back({i, 0, 0, 0});
+        p.empty++;
+    }
     std::vector<int> next(first.begin(), first.end() - 1);
     for (const PageItem &it : p.items) {
         if (it.unit < 0) continue;

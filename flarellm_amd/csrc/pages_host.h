@@ -104,8 +104,10 @@ struct PagePlan {
     bool wide = false;            // an item of a form above 0
     std::vector<PageQuery> order;
     std::vector<int> page_ids, units;
-    std::vector<PageJoin> joins;
-    int num_units = 0;
+    std::vector<PageJoin> joins;  // those without partial results last
+    std::vector<int> join_of;     // of each query (-1: none)
+    int num_units = 0, empty = 0; // joins without partial results
+    int most_parts = 0, most_queries = 0;  // of a join; of an item with partial results
 };
 
 // seen[i] tokens of sequence s[i] for query i (checked against the table).

@@ -412,10 +412,17 @@ __device__ __forceinline__ PageItem pg_item(const PageAttnArgs &a, int i) {
     return PageItem{w[0], w[1], w[2], w[3], w[4], w[5], w[6], w[7]};
 }
 
+// A value of a partial result.  HERE: another workgroup of the launch reads it.
+template <bool HERE>
+__device__ __forceinline__ void pg_put(float *p, float v) {
+    if constexpr (HERE) st_agent(p, v);
+    else *p = v;
+}
+
 // An item's rows key by key, where some value was not finite: 2^kShift times the
 // sum and O, in base 2 relative to the largest score, as the tiles have them (all rows
 // of the item; this is rare).  lds: 260 floats.
-template <int FMT, int D>
+template <int FMT, int D, bool HERE>
 __device__ __forceinline__ void pg_rows_again(const PageAttnArgs &a, const PageItem &it, int kvh, float *lds) {
     const int nkv = a.pool.nkv, G = a.group, nh = nkv * G, P = a.pool.P, rows = it.nq * G;
     const size_t layer_pages = (size_t)a.layer * a.pool.pages;
@@ -458,10 +465,10 @@ __device__ __forceinline__ void pg_rows_again(const PageAttnArgs &a, const PageI
             a.out[((size_t)pq.query * nh + hd) * D + tid] = acc / sum;
         } else {
             const size_t u = (size_t)(it.unit + qi) * nh + hd;
-            a.part[u * D + tid] = acc;
+            pg_put<HERE>(a.part + u * D + tid, acc);
             if (tid == 0) {
-                a.ml[u * 2] = mx;
-                a.ml[u * 2 + 1] = sum;
+                pg_put<HERE>(a.ml + u * 2, mx);
+                pg_put<HERE>(a.ml + u * 2 + 1, sum);
             }
         }
     }
@@ -483,7 +490,7 @@ __device__ __forceinline__ void pg_stage_q(const PageAttnArgs &a, const PageItem
 
 // A row of an item's result: channels ch .. ch + 3 from the KL partial results at
 // lds[i * step], each [D] O, max, sum.  Sets *bad where a value is not finite.
-template <int D, int KL>
+template <int D, int KL, bool HERE>
 __device__ __forceinline__ void pg_join_row(const PageAttnArgs &a, const PageItem &it, int kvh, int row, int ch,
                                             const float *lds, int step, int *bad) {
     float mx = -INFINITY, sum = 0.0f, wt[KL];
@@ -512,10 +519,15 @@ __device__ __forceinline__ void pg_join_row(const PageAttnArgs &a, const PageIte
         y[k] *= il;
         odd = __builtin_fmaf(y[k], 0.0f, odd);
     }
-    *(pf4_t *)op = y;
+    if (!HERE || it.unit < 0) {
+        *(pf4_t *)op = y;
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; k++) st_agent(op + k, y[k]);
+    }
     if (it.unit >= 0 && ch == 0) {
-        a.ml[u * 2] = mx;
-        a.ml[u * 2 + 1] = sum;
+        pg_put<HERE>(a.ml + u * 2, mx);
+        pg_put<HERE>(a.ml + u * 2 + 1, sum);
     }
     if (odd != 0.0f) *bad = 1;  // 0 * Inf and 0 * NaN are NaN
 }
@@ -530,7 +542,7 @@ __device__ __forceinline__ void pg_join_row(const PageAttnArgs &a, const PageIte
 // a token that some of the item's queries see and others do not has p = 0 for the
 // latter, and 0 * Inf is NaN, as is an Inf against a zero low part.  Every such case
 // leaves a NaN or Inf in O: such a row is then formed again, key by key.
-template <int FMT, int D, int NT, int NW>
+template <int FMT, int D, int NT, int NW, bool HERE>
 __device__ __forceinline__ void pg_narrow(const PageAttnArgs &a, const PageItem &it, int kvh, float *lds, int *bad) {
     using Block = PgBlock<FMT, D>;
     constexpr bool QL = pg_q_in_lds(FMT, D, NT);
@@ -662,7 +674,7 @@ __device__ __forceinline__ void pg_narrow(const PageAttnArgs &a, const PageItem 
         }
         __syncthreads();
         for (int r = threadIdx.x / (D / 4); r < min(16, rows - 16 * n); r += 64 * NW / (D / 4))
-            pg_join_row<D, NW>(a, it, kvh, 16 * n + r, threadIdx.x % (D / 4) * 4, lds + r * LROW, 16 * LROW, bad);
+            pg_join_row<D, NW, HERE>(a, it, kvh, 16 * n + r, threadIdx.x % (D / 4) * 4, lds + r * LROW, 16 * LROW, bad);
     }
 }
 
@@ -672,7 +684,7 @@ __device__ __forceinline__ void pg_narrow(const PageAttnArgs &a, const PageItem 
 // 32 x 32 x 16: a query row is a lane (mod 32), the K rows enter with index bits 2 and 3
 // swapped so that scores i = 8 mm + j of a lane are slots 16 mm + 8 (lane / 32) + j, the
 // operand of O^T = V^T P^T.  smem: two steps of K and V; at the end [8][32][D + 4] floats.
-template <int D, int R>
+template <int D, int R, bool HERE>
 __device__ __forceinline__ void pg_wide(const PageAttnArgs &a, const PageItem &it, int kvh, char *smem, int *bad) {
     constexpr int FMT = FL_KV_F16, KL = 8 / R, NB = 4 / KL;
     constexpr int KS = D / 16, DT = D / 32, CH = D / 8, BLK = 32 * D * 2;  // BLK: bytes of a block's K (or V)
@@ -847,41 +859,115 @@ __device__ __forceinline__ void pg_wide(const PageAttnArgs &a, const PageItem &i
     }
     __syncthreads();
     for (int r = threadIdx.x / (D / 4); r < rows; r += 512 / (D / 4))
-        pg_join_row<D, KL>(a, it, kvh, r, threadIdx.x % (D / 4) * 4, lds + (size_t)r * LROW, 32 * R * LROW, bad);
+        pg_join_row<D, KL, HERE>(a, it, kvh, r, threadIdx.x % (D / 4) * 4, lds + (size_t)r * LROW, 32 * R * LROW, bad);
+}
+
+// Partial results of a query and head, N of them in flight, into o, l relative to mx
+struct PgSum {
+    float mx = -INFINITY, l = 0.0f;
+    pf4_t o = {0, 0, 0, 0};
+    // parts first, first + step, ..; value(unit index, ml, o)
+    template <int N, typename F>
+    __device__ __forceinline__ void add(int first, int end, int step, F value) {
+        for (int i = first; i < end; i += step * N) {
+            float2 ml[N];
+            pf4_t p[N];
+#pragma unroll
+            for (int k = 0; k < N; k++) value(min(i + step * k, end - 1), ml[k], p[k]);
+            float mn = mx;
+#pragma unroll
+            for (int k = 0; k < N; k++) mn = fmaxf(mn, ml[k].x);
+            const float al = mx == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mx - mn);
+            mx = mn;
+            l *= al;
+#pragma unroll
+            for (int x = 0; x < 4; x++) o[x] *= al;
+#pragma unroll
+            for (int k = 0; k < N; k++) {
+                if (i + step * k >= end) break;
+                const float w = ml[k].x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml[k].x - mx);
+                l = __builtin_fmaf(ml[k].y, w, l);
+#pragma unroll
+                for (int x = 0; x < 4; x++) o[x] = __builtin_fmaf(p[k][x], w, o[x]);
+            }
+        }
+    }
+};
+
+// At the end of an item: joins the queries of which this workgroup has the last part for
+// its kv head to arrive, in the order of the plan whichever that is.  Parts are stored and
+// read past the XCDs' caches (st_agent, ld_agent), a wave's before its workgroup counts.
+// last: NTHR / 4 ints of LDS (an item has as many queries at most).
+template <int D, int NTHR>
+__device__ __forceinline__ void pg_join_here(const PageAttnArgs &a, const PageItem &it, int kvh, int *last) {
+    const int nkv = a.pool.nkv, G = a.group, nh = nkv * G, tid = threadIdx.x;
+    if (blockIdx.x < (unsigned)nkv)
+        for (int i = tid; i < a.nempty * G * D; i += NTHR)
+            a.out[((size_t)a.joins[a.njoins - 1 - i / (G * D)].query * nh + kvh * G) * D + i % (G * D)] = 0.0f;
+    if (it.unit < 0) return;
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    if (tid < it.nq) {
+        const int j = a.join_of[a.order[it.q0 + tid].query];
+        int *c = a.arrived + (size_t)j * nkv + kvh;
+        const bool mine = __hip_atomic_fetch_add(c, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == a.joins[j].count - 1;
+        if (mine) __hip_atomic_store(c, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        last[tid] = mine ? j : -1;
+    }
+    __syncthreads();
+    const int per = G * (D / 4);  // threads of a query
+    for (int i = tid; i < it.nq * per; i += NTHR) {
+        const int qi = i / per, e = i - qi * per, hd = kvh * G + e / (D / 4), ch = e % (D / 4) * 4;
+        if (last[qi] < 0) continue;
+        const PageJoin j = a.joins[last[qi]];
+        PgSum s;
+        s.add<8>(0, j.count, 1, [&](int k, float2 &ml, pf4_t &p) {
+            const size_t u = (size_t)a.units[j.first + k] * nh + hd;
+            ml = ld_agent2(a.ml + u * 2);
+            const float2 x = ld_agent2(a.part + u * D + ch), y = ld_agent2(a.part + u * D + ch + 2);
+            p = pf4_t{x.x, x.y, y.x, y.y};
+        });
+        const float il = 1.0f / s.l;
+        *(pf4_t *)(a.out + ((size_t)j.query * nh + hd) * D + ch) = pf4_t{s.o[0] * il, s.o[1] * il, s.o[2] * il, s.o[3] * il};
+    }
 }
 
 // One item (PageItem) and kv head per workgroup; the kv head is the faster index, so that
 // with 8 of them the items of a head share an XCD's L2.
 
-// Items of up to 16 rows (FORMS = 1), or up to 32: 4 waves.
-template <int FMT, int D, int FORMS>
+// Items of up to 16 rows (FORMS = 1), or up to 32: 4 waves.  HERE: partial results are joined in
+// the launch (a kernel of its own: with the code of it, but not taken, 32 sequences over 8 bits
+// 25.2 us against 24.4).
+template <int FMT, int D, int FORMS, bool HERE>
 __global__ __launch_bounds__(256, page_waves(FMT, D, FORMS)) void k_pages_attn(PageAttnArgs a) {
     __shared__ __align__(16) float lds[4 * 16 * (D + 4) + (pg_q_in_lds(FMT, D, FORMS) ? FORMS * PgBlock<FMT, D>::QP * 256 : 0)];
     __shared__ int bad;
     const int kvh = blockIdx.x % a.pool.nkv;
     const PageItem it = pg_item(a, blockIdx.x / a.pool.nkv);
     if (threadIdx.x == 0) bad = 0;
-    if (FORMS == 1 || it.form == 0) pg_narrow<FMT, D, 1, 4>(a, it, kvh, lds, &bad);
-    else pg_narrow<FMT, D, FORMS, 4>(a, it, kvh, lds, &bad);
+    if (FORMS == 1 || it.form == 0) pg_narrow<FMT, D, 1, 4, HERE>(a, it, kvh, lds, &bad);
+    else pg_narrow<FMT, D, FORMS, 4, HERE>(a, it, kvh, lds, &bad);
     __syncthreads();
-    if (bad) pg_rows_again<FMT, D>(a, it, kvh, lds);
+    if (bad) pg_rows_again<FMT, D, HERE>(a, it, kvh, lds);
+    if constexpr (HERE) pg_join_here<D, 256>(a, it, kvh, (int *)lds);
 }
 
 // binary16, items of up to 128 rows: 8 waves, one workgroup a CU.  (In one launch, so that
 // items of many rows, which the matrix cores bound, run beside those of few, which the
 // memory does.)
-template <int D>
+template <int D, bool HERE>
 __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) void k_pages_attn_wide(PageAttnArgs a) {
     extern __shared__ __align__(16) char smem[];
     __shared__ int bad;
     const int kvh = blockIdx.x % a.pool.nkv;
     const PageItem it = pg_item(a, blockIdx.x / a.pool.nkv);
     if (threadIdx.x == 0) bad = 0;
-    if (it.form == 0) pg_narrow<FL_KV_F16, D, 1, 8>(a, it, kvh, (float *)smem, &bad);
-    else if (it.form == 1) pg_wide<D, 2>(a, it, kvh, smem, &bad);
-    else pg_wide<D, 4>(a, it, kvh, smem, &bad);
+    if (it.form == 0) pg_narrow<FL_KV_F16, D, 1, 8, HERE>(a, it, kvh, (float *)smem, &bad);
+    else if (it.form == 1) pg_wide<D, 2, HERE>(a, it, kvh, smem, &bad);
+    else pg_wide<D, 4, HERE>(a, it, kvh, smem, &bad);
     __syncthreads();
-    if (bad) pg_rows_again<FL_KV_F16, D>(a, it, kvh, (float *)smem);
+    if (bad) pg_rows_again<FL_KV_F16, D, HERE>(a, it, kvh, (float *)smem);
+    if constexpr (HERE) pg_join_here<D, 512>(a, it, kvh, (int *)smem);
 }
 
 // Partial results of a query joined: a workgroup takes 128 channels, 4 a thread, and
@@ -895,40 +981,18 @@ __global__ __launch_bounds__(256) void k_pages_join(PageJoinArgs a) {
     const PageJoin j = a.joins[blockIdx.x];
     const int c = threadIdx.x & 31, s = threadIdx.x >> 5;
     const int e = blockIdx.y * 128 + 4 * c, ec = min(e, a.heads * D - 4), hd = ec / D, n = j.count;
-    float mx = -INFINITY, l = 0.0f;
-    pf4_t o = {0, 0, 0, 0};
-    for (int i = s; i < n; i += 8 * U) {
-        float mi[U], li[U];
-        pf4_t p[U];
-#pragma unroll
-        for (int k = 0; k < U; k++) {
-            const size_t u = (size_t)a.units[j.first + min(i + 8 * k, n - 1)] * a.heads + hd;
-            mi[k] = a.ml[u * 2];
-            li[k] = a.ml[u * 2 + 1];
-            p[k] = *(const pf4_t *)(a.part + u * D + ec % D);
-        }
-        float mn = mx;
-#pragma unroll
-        for (int k = 0; k < U; k++) mn = fmaxf(mn, mi[k]);
-        const float al = mx == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mx - mn);
-        mx = mn;
-        l *= al;
-#pragma unroll
-        for (int k = 0; k < 4; k++) o[k] *= al;
-#pragma unroll
-        for (int k = 0; k < U; k++) {
-            if (i + 8 * k >= n) break;
-            const float w = mi[k] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mi[k] - mx);
-            l = __builtin_fmaf(li[k], w, l);
-#pragma unroll
-            for (int x = 0; x < 4; x++) o[x] = __builtin_fmaf(p[k][x], w, o[x]);
-        }
-    }
-    *(pf4_t *)lds[s][c] = o;
-    lml[s][c][0] = mx;
-    lml[s][c][1] = l;
+    PgSum part;
+    part.add<U>(s, n, 8, [&](int i, float2 &ml, pf4_t &p) {
+        const size_t u = (size_t)a.units[j.first + i] * a.heads + hd;
+        ml = *(const float2 *)(a.ml + u * 2);
+        p = *(const pf4_t *)(a.part + u * D + ec % D);
+    });
+    *(pf4_t *)lds[s][c] = part.o;
+    lml[s][c][0] = part.mx;
+    lml[s][c][1] = part.l;
     __syncthreads();
     if (s) return;
+    float mx = part.mx, l;
     for (int i = 1; i < 8; i++) mx = fmaxf(mx, lml[i][c][0]);
     float y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     l = 0.0f;

@@ -375,6 +375,43 @@ def test_an_extend_that_fails_leaves_the_one_before(backend):
     t.check_rows()
 
 
+@pytest.mark.parametrize("fmt,heads,kv_heads,D", [("f32", 9, 3, 64), ("f16", 32, 8, 128), ("q8", 8, 8, 64), ("f16", 14, 2, 64)])
+def test_joined_where_the_last_part_arrives(backend, fmt, heads, kv_heads, D):
+    """A few parts a query, joined in the launch: in the same order whichever arrives last, call after
+    call with one plan (its counts start from zero again) and with others between; queries that see nothing."""
+    t = Twin(backend, fmt, heads, kv_heads, D, 32, 200, seqs=12, max_len=2000, seed=heads)
+    t.extend([0], [700])
+    t.fork([0] * 5, [1, 2, 3, 4, 5], [700, 690, 512, 100, 700])
+    t.extend([0, 1, 2, 3, 6], [9, 60, 33, 1, 400])
+    seqs, seen = [0, 1, 2, 3, 4, 5, 6, 7, 5, 1, 8], [709, 760, 723, 513, 100, 0, 400, 0, 31, 650, 0]
+    q = t.rng.standard_normal((len(seqs), heads, D)).astype(np.float32)
+    first = t.check(seqs, seen, q=q)
+    for i in range(20):
+        got = t.check(seqs, seen, q=q)
+        assert np.array_equal(got, first)
+        if i % 5 == 0:
+            t.check([1, 6], [760, 399])
+    many = [s for s in range(7) for _ in range(40)]  # joined by a launch of its own
+    t.check(many, [100 - i % 40 for i in range(len(many))])
+    t.check(many, [t.rows[s][0].shape[1] - i % 40 for i, s in enumerate(many)])
+    assert np.array_equal(t.check(seqs, seen, q=q), first)
+
+
+def test_values_not_finite_in_a_part(backend):
+    """An infinity in one part of a query that others do not see."""
+    t = Twin(backend, "f16", 8, 2, 64, 32, 60, seqs=4)
+    k, v = (t.rng.standard_normal((1, 600, 2, 64)).astype(np.float32) for _ in "kv")
+    v[0, 300, 1, 5] = np.inf
+    t.extend([0], [600], (k, v))
+    t.fork([0], [1], [290])
+    t.extend([1], [50])
+    q = t.rng.standard_normal((3, 8, 64)).astype(np.float32)
+    got, want, tol = t.attend([0, 1, 0], [600, 340, 300], q=q)
+    assert np.isposinf(got[0, 4:, 5]).all()
+    got[0, 4:, 5] = want[0, 4:, 5] = tol[0, 4:, 5] = 0
+    assert (np.abs(got - want) <= tol).all()
+
+
 def test_one_token_of_many_layers(backend):
     """A token of a [layers, tokens, ..] buffer; a page's last slots."""
     t = Twin(backend, "f32", 4, 2, 64, 32, 20, layers=4)
