@@ -299,13 +299,15 @@ PageForms forms_of(const fl_pages *p) {
 // against 17.7).  With more it goes over them again and again, past the caches: two times 8 of
 // 4 sequences behind 1774 tokens 19.2 against 17.6, 16 sequences of up to 8000 45.4 against 41.7,
 // 32 in a tree 44 against 24; and stores past the caches cost more than those that
-// stay: 644 queries, 10 MB, 62.2 against 58.5.
+// stay: 644 queries, 10 MB, 62.2 against 58.5.  (One workgroup a kv head clears the rows of
+// queries that see nothing: few.)
 bool joins_here(const fl_pages *p, int heads) {
     const PagePlan &l = p->plan;
     const int threads = l.wide && p->cfg.kv_format == FL_KV_F16 ? 512 : 256;
     const int rows = l.most_queries * (heads / p->cfg.num_kv_heads);
     const long long rounds = (rows * (p->cfg.head_dim / 4) + threads - 1) / threads;
-    return !l.items.empty() && rounds * l.most_parts <= 8 && (long long)l.num_units * heads * p->cfg.head_dim <= (1 << 18);
+    return !l.items.empty() && l.empty <= 64 && rounds * l.most_parts <= 8 &&
+           (long long)l.num_units * heads * p->cfg.head_dim <= (1 << 18);
 }
 
 // The plan of these queries, on the device.

@@ -65,6 +65,7 @@ class PagedKv:
         self._stream = self.stream.cuda_stream
         self._current, self._index = torch._C._cuda_getCurrentRawStream, self.device.index
         self._row = (kv_heads, head_dim)
+        self._torch = torch  # (an import statement costs a call 0.3 us)
         self._before, self._behind = torch.cuda.Event(), torch.cuda.Event()  # (kept: making one costs 10 us)
         # the memory may be what earlier work of the current stream still uses
         self.stream.wait_stream(torch.cuda.current_stream(self.device))
@@ -100,8 +101,7 @@ class PagedKv:
         """_call behind the current torch stream's work, and before what follows there."""
         if self._current(self._index) == self._stream:
             return self._call(fn, *args)
-        import torch
-
+        torch = self._torch
         current = torch.cuda.current_stream(self.device)
         self._before.record(current)
         self.stream.wait_event(self._before)
@@ -113,9 +113,8 @@ class PagedKv:
 
     def _rows(self, t, what: str, shape):
         """A float32 tensor on this device whose last dimensions are `shape`, without gaps between them."""
-        import torch
-
-        if not isinstance(t, torch.Tensor) or t.dtype is not torch.float32 or t.device != self.device:
+        torch = self._torch
+        if not isinstance(t, torch.Tensor) or t.dtype is not torch.float32 or t.get_device() != self._index:
             raise ValueError(f"{what}: a float32 tensor on {self.device}")
         n = len(shape)
         if t.shape[-n:] != shape:
@@ -214,8 +213,7 @@ class PagedKv:
 
     def read(self, seqs, starts, counts, layer: int = 0):
         """The f32 keys and values [tokens, kv_heads, head_dim] of counts[i] tokens of each sequence, from starts[i] on."""
-        import torch
-
+        torch = self._torch
         seqs = _ids(seqs, "seqs")
         starts, counts = _ids(starts, "starts", seqs.size), _ids(counts, "counts", seqs.size)
         shape = (max(0, int(counts.sum())), self.kv_heads, self.head_dim)
@@ -227,8 +225,7 @@ class PagedKv:
     def attention(self, q, seqs, seen=None, layer: int = 0, out=None):
         """Attention of queries q [n, heads, head_dim] (RoPE applied; rows may be slices of wider ones): query i
         over the first seen[i] tokens (all of them) of sequence seqs[i].  -> [n, heads, head_dim] (out: apart from q)"""
-        import torch
-
+        torch = self._torch
         if not isinstance(q, torch.Tensor) or q.dim() != 3:
             raise ValueError("q: [n, heads, head_dim]")
         n, heads, _ = shape = q.shape

@@ -397,6 +397,20 @@ def test_joined_where_the_last_part_arrives(backend, fmt, heads, kv_heads, D):
     assert np.array_equal(t.check(seqs, seen, q=q), first)
 
 
+@pytest.mark.parametrize("idle", [1, 64, 65, 3000])
+def test_queries_that_see_nothing(backend, idle):
+    """Rows of empty sequences among others are zeros, wherever and however many they are."""
+    t = Twin(backend, "f16", 4, 2, 64, 32, 40, seqs=8)
+    t.extend([0, 1], [500, 3])
+    for rest in ([0], [1], [0, 1, 1], []):
+        seqs = [2] * (idle // 2) + rest + [3] * (idle - idle // 2)
+        out = torch.full((len(seqs), 4, 64), float("nan"), device="cuda")
+        q = t.rng.standard_normal((len(seqs), 4, 64)).astype(np.float32)
+        t.check(seqs, q=q, out=out)
+        empty = [i for i, s in enumerate(seqs) if s > 1]
+        assert not out[empty].any()
+
+
 def test_values_not_finite_in_a_part(backend):
     """An infinity in one part of a query that others do not see."""
     t = Twin(backend, "f16", 8, 2, 64, 32, 60, seqs=4)
