@@ -298,7 +298,9 @@ PageForms forms_of(const fl_pages *p) {
 // of 5 sequences 14.4 against 17.0, 21 sequences behind 595 tokens, two times 4 a thread, 15.4
 // against 17.7).  With more it goes over them again and again, past the caches: two times 8 of
 // 4 sequences behind 1774 tokens 19.2 against 17.6, 16 sequences of up to 8000 45.4 against 41.7,
-// 32 in a tree 44 against 24; and stores past the caches cost more than those that
+// 32 in a tree 44 against 24.  (Calls one after another, which the host's launches bound; the
+// GPU alone takes 11.6 us for the 8 answers against 9.4 with the second launch: the stores past the
+// caches, the count and the loads behind it are a chain of 4 us.)  And stores past the caches cost more than those that
 // stay: 644 queries, 10 MB, 62.2 against 58.5.  (One workgroup a kv head clears the rows of
 // queries that see nothing: few.)
 bool joins_here(const fl_pages *p, int heads) {
