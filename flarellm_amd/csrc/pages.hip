@@ -477,7 +477,8 @@ int fl_pages_extend(fl_pages *p, const int32_t *seqs, const int32_t *counts, int
     if (most > kMaxGrid) return fail(p, FL_E_INVALID, "too many tokens at once");
     DevBuf more;
     const size_t bytes = most > kInlineRuns ? (size_t)most * sizeof(PageRun) : 0;
-    int rc = copies_room(p, bytes ? 1 : 0, n);
+    int rc = copies_room(p, 0, n);  // (the first to be sent, or behind the runs)
+    if (!rc && bytes) rc = copies_room(p, 1, n);
     if (!rc && bytes) rc = stage_room(p, 0, bytes);
     if (!rc && bytes > p->d_runs.cap) rc = ensure(p, more, std::max(bytes, 2 * p->d_runs.cap));
     if (!rc) rc = on_table(p, [&](PageTable &t) { return t.extend(seqs, counts, n); });

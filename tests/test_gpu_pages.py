@@ -426,6 +426,25 @@ def test_values_not_finite_in_a_part(backend):
     assert (np.abs(got - want) <= tol).all()
 
 
+@pytest.mark.parametrize("new", [1, 70])
+def test_long_lists(backend, new):
+    """More copies and runs of one call than go with its launch, and the two lists together."""
+    t = Twin(backend, "f16", 2, 1, 64, 64, 700, seqs=130, max_len=12000, layers=2)
+    t.extend([0], [9 * 64 + 20])
+    t.fork([0] * 129, list(range(1, 130)))
+    t.extend(list(range(130)), [new] * 130)
+    t.check_rows()
+    t.check(list(range(0, 130, 9)), layer=1)
+    t.truncate(list(range(130)), [9 * 64] * 130)
+    t.free(list(range(1, 129)))
+    t.extend([0], [7000])
+    t.fork([0, 129], [1, 2], deep=True)
+    t.free([0])
+    assert t.kv.compact() > 96
+    t.check_rows()
+    t.check([1, 2, 129], layer=1)
+
+
 def test_one_token_of_many_layers(backend):
     """A token of a [layers, tokens, ..] buffer; a page's last slots."""
     t = Twin(backend, "f32", 4, 2, 64, 32, 20, layers=4)
